@@ -72,6 +72,8 @@ typedef enum {
 #define LMCB_DEVICE_FLAG_STREAM_OVERFLOW 0x4u
 #define LMCB_DEVICE_FLAG_WAIT_TIMEOUT 0x8u
 #define LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE 0x10u
+#define LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE 0x20u
+#define LMCB_DEVICE_FLAG_PAGES_EXHAUSTED 0x40u
 
 /* Library version, "major.minor.patch". */
 LMCB_API const char* lmcb_version(void);
@@ -362,6 +364,134 @@ LMCB_API int lmcb_rotary_embedding_k_fused(const void* oldPositions, const void*
                                            const void* cosSinCache, int cacheType,
                                            int64_t rotDim, int64_t maxPosition, int isNeox,
                                            void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Serving operators around the paged cache                                   */
+/* ------------------------------------------------------------------------- */
+/* None of these has a reference counterpart: they make the slot mappings the
+ * transfers take, the keys the cache holds, and a cache in 4 bits with the
+ * attention that reads it. All are asynchronous on `stream`, allocate nothing
+ * and can be captured in a CUDA graph. */
+
+/* Block tables, slot mapping, positions and lengths of a batch from its
+ * request lengths, in one launch. Request b has contextLens[b] tokens in the
+ * cache and brings queryLens[b] new ones; pages hold blockSize tokens. Its new
+ * pages are the next ones of freeBlocks, requests in order, and go into its row
+ * of blockTable behind the ceil(contextLens[b] / blockSize) entries that it
+ * has; entries behind those are left as they were.
+ *   contextLens, queryLens  [numRequests] of lenType (INT32 or INT64)
+ *   blockTable     [numRequests, tableCols] int32, rows tableStride apart,
+ *                  read and written; tableCols * blockSize < 2^31
+ *   freeBlocks     [numFree] int32
+ *   slotMapping, positions  [numTokens] of slotType, out. Token i of request b
+ *                  is entry queryStart[b] + i: its position is contextLens[b] +
+ *                  i, its slot page * blockSize + position % blockSize, or -1
+ *                  (which the transfers skip) where it has no page. Entries
+ *                  behind the last request: slot -1, position 0.
+ *   queryStart     [numRequests + 1] int32, out: first entry of each request
+ *   seqLens        [numRequests] int32, out: contextLens + queryLens
+ *   blocksUsed     [1] int32, out: entries of freeBlocks that were asked for
+ * A free list that runs out gives table entries and slots of -1 and sets
+ * LMCB_DEVICE_FLAG_PAGES_EXHAUSTED, as tokens behind a table row's end do.
+ * Negative lengths count as 0, and tokens that do not fit numTokens are left
+ * out (queryStart stops at numTokens); both set
+ * LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE. At most 16384 requests
+ * (LMCB_ERR_CAPACITY). No output may overlap an input or another output. */
+LMCB_API int lmcb_build_slot_mapping(const void* contextLens, const void* queryLens, int lenType,
+                                     int32_t numRequests, int32_t* blockTable,
+                                     int64_t tableStride, int32_t tableCols,
+                                     const int32_t* freeBlocks, int64_t numFree,
+                                     int32_t blockSize, int64_t numTokens, void* slotMapping,
+                                     void* positions, int slotType, int32_t* queryStart,
+                                     int32_t* seqLens, int32_t* blocksUsed, void* stream);
+
+/* RMS norm of every query and key head with the position rotation in the same
+ * pass: y = x / sqrt(mean(x^2) + eps) * weight, then the first rotDim values
+ * rotated by the angles of the token's position, in fp32, rounded once.
+ *   query, key     [numTokens, heads, headSize] of `type`; tokens
+ *                  *TokenStride elements apart (>= heads * headSize), so both
+ *                  may be parts of one packed projection
+ *   queryWeight, keyWeight  [headSize] of their types, NULL for none
+ *   cosSinCache, isNeox     as in lmcb_rotary_embedding_k_fused
+ *   queryOut, keyOut        as query and key; each may be its input itself
+ * Positions outside [0, maxPosition) leave their token's output as it was and
+ * set LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE. */
+LMCB_API int lmcb_qk_norm_rope(const void* query, const void* key, int type,
+                               int64_t queryTokenStride, int64_t keyTokenStride,
+                               const void* queryWeight, int queryWeightType,
+                               const void* keyWeight, int keyWeightType, const void* positions,
+                               int posType, const void* cosSinCache, int cacheType,
+                               int64_t rotDim, int64_t maxPosition, int isNeox, double eps,
+                               int64_t numTokens, int64_t numQueryHeads, int64_t numKeyHeads,
+                               int64_t headSize, void* queryOut, int64_t queryOutStride,
+                               void* keyOut, int64_t keyOutStride, void* stream);
+
+/* The paged KV cache held in 4 bits: int32 [2, numBlocks, blockSize, W], K
+ * rows then V rows. A row of H heads of D values holds H * D / 8 words of codes
+ * (word h * D / 8 + w: values 8 w ... 8 w + 7 of head h, value 8 w + j in bits
+ * 4 j ... 4 j + 3), then one word a head: fp16 scale s in the low half, fp16
+ * zero z in the high half. A code c stands for z + s c, with z = fp16(min),
+ * s = fp16((max - min) / 15) of the head's values and the nearest code, ties
+ * to even; NaN is kept as 0, values beyond the fp16 range as its ends. W is
+ * that length rounded up to four words, so a 4-bit cache moves through the
+ * transfers above as rows of W int32 (type LMCB_DTYPE_INT32, hiddenDims W). */
+
+/* W, or 0 for a head size that is not a multiple of 8 up to 256. */
+LMCB_API int64_t lmcb_kv4_row_words(int64_t numHeads, int64_t headSize);
+
+/* Rounds key and value [numTokens, numHeads, headSize] (fp32, bf16 or fp16;
+ * tokens *TokenStride elements apart) to 4 bits, into the rows of slotMapping.
+ * Slots < 0 are skipped; slots beyond the cache are skipped and set
+ * LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE. The slots of a call are distinct. */
+LMCB_API int lmcb_kv4_store(const void* key, const void* value, int type, int64_t keyTokenStride,
+                            int64_t valueTokenStride, int32_t* kvCache, int64_t numBlocks,
+                            int64_t blockSize, const void* slotMapping, int slotType,
+                            int64_t numTokens, int64_t numHeads, int64_t headSize, void* stream);
+
+/* The values of the rows of slotMapping, in fp32, bf16 or fp16. Rows of
+ * skipped slots (as in lmcb_kv4_store) are left as they were. */
+LMCB_API int lmcb_kv4_load(const int32_t* kvCache, int64_t numBlocks, int64_t blockSize,
+                           const void* slotMapping, int slotType, void* key, void* value,
+                           int type, int64_t keyTokenStride, int64_t valueTokenStride,
+                           int64_t numTokens, int64_t numHeads, int64_t headSize, void* stream);
+
+/* Attention of a batch over its 4-bit pages.
+ *   query, out     [numQueryRows, numQueryHeads, headSize] bf16 or fp16, tokens
+ *                  *TokenStride elements apart; headSize 64, 128 or 256
+ *   blockTable     [batch, tableCols] int32, rows tableStride apart
+ *   seqLens        [batch] int32: tokens in the cache, the queries' own among them
+ *   queryStart     [batch + 1] int32: request b's queries are rows
+ *                  queryStart[b] ... queryStart[b + 1], the last of them at
+ *                  position seqLens[b] - 1. NULL: row b is request b's one query.
+ *   maxQueryLen    no request has more queries (a larger one is left out and flagged)
+ *   maxSeqLen      how long requests are expected to be: sizes the launch only
+ *   scale          factor of q . k before the softmax
+ *   window, sinks  window > 0: a query sees the last `window` keys up to its own
+ *                  and the first `sinks` keys; window 0: all keys up to its own
+ *   workspace      lmcb_kv4_attention_workspace bytes (the same sizes), 16-byte
+ *                  aligned; NULL where that is 0. Calls that may overlap on the
+ *                  GPU need one each.
+ * A query that sees no key gets zeros. Rows behind the last request are left as
+ * they were. Keys on pages outside the cache are not seen and set
+ * LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE; lengths outside [0, tableCols * blockSize]
+ * count as 0, and a queryStart that leaves [0, numQueryRows] or descends gives
+ * its request no queries; both set LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE. */
+LMCB_API int lmcb_kv4_attention(const void* query, int type, int64_t queryTokenStride,
+                                int64_t numQueryRows, const int32_t* kvCache, int64_t numBlocks,
+                                int64_t blockSize, const int32_t* blockTable, int64_t tableStride,
+                                int64_t tableCols, const int32_t* seqLens,
+                                const int32_t* queryStart, int64_t batch, int64_t maxQueryLen,
+                                int64_t maxSeqLen, int64_t numKvHeads, int64_t numQueryHeads,
+                                int64_t headSize, double scale, int64_t window, int64_t sinks,
+                                void* out, int64_t outTokenStride, void* workspace,
+                                size_t workspaceBytes, void* stream);
+
+/* Bytes of workspace that lmcb_kv4_attention needs for these sizes on the
+ * current device. */
+LMCB_API int lmcb_kv4_attention_workspace(int64_t batch, int64_t maxQueryLen, int64_t maxSeqLen,
+                                          int64_t numKvHeads, int64_t numQueryHeads,
+                                          int64_t headSize, int64_t window, int64_t sinks,
+                                          size_t* bytesOut);
 
 #ifdef __cplusplus
 }  /* extern "C" */

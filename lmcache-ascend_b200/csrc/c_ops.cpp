@@ -15,9 +15,11 @@
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "lmcache_b200.h"
@@ -675,6 +677,282 @@ void rotary_embedding_k_fused(const torch::Tensor& old_positions,
       cos_sin_cache.size(0), is_neox ? 1 : 0, current_stream()));
 }
 
+// ---------------------------------------------------------------------------
+// Serving operators around the paged cache (additions to the reference surface)
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// Bytes [first, last) that a tensor of non-negative strides may touch.
+std::pair<uintptr_t, uintptr_t> byte_range(const torch::Tensor& t) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {first, first};
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {first, first + static_cast<uintptr_t>((last + 1) * t.element_size())};
+}
+
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  const auto x = byte_range(a), y = byte_range(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+void check_cuda(const torch::Tensor& t, const torch::Device& dev, const char* who,
+                const char* name) {
+  TORCH_CHECK(t.is_cuda(), who, ": ", name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == dev, who, ": ", name, " is on ", t.device(), ", expected ", dev);
+}
+
+// A contiguous vector of one of the index types.
+void check_index(const torch::Tensor& t, const torch::Device& dev, const char* who,
+                 const char* name, int64_t size, bool int32_only) {
+  check_cuda(t, dev, who, name);
+  TORCH_CHECK(t.dim() == 1 && t.is_contiguous() && t.size(0) == size, who, ": ", name,
+              " must be a contiguous vector of ", size, " entries");
+  TORCH_CHECK(t.scalar_type() == at::kInt || (!int32_only && t.scalar_type() == at::kLong), who,
+              ": ", name, int32_only ? " must be int32" : " must be int32 or int64");
+}
+
+// Head rows [num_tokens, heads, head_size], dense within a token.
+void check_heads(const torch::Tensor& t, const torch::Device& dev, const char* who,
+                 const char* name) {
+  check_cuda(t, dev, who, name);
+  TORCH_CHECK(t.dim() == 3, who, ": ", name, " must be [num_tokens, heads, head_size]");
+  TORCH_CHECK((t.size(2) == 1 || t.stride(2) == 1) &&
+                  (t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
+                  (t.size(0) <= 1 || t.stride(0) >= t.size(1) * t.size(2)),
+              who, ": ", name, " must be dense within a token");
+}
+
+int64_t token_stride(const torch::Tensor& t) {
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+}
+
+// A layer's 4-bit cache, int32 [2, num_blocks, block_size, ...] with rows of
+// kv4_row_words(heads, head_size) words.
+void check_kv4_cache(const torch::Tensor& cache, const torch::Device& dev, const char* who,
+                     int64_t heads, int64_t head_size) {
+  check_cuda(cache, dev, who, "kv_cache");
+  TORCH_CHECK(cache.scalar_type() == at::kInt, who, ": kv_cache must be int32");
+  TORCH_CHECK(cache.dim() >= 4 && cache.size(0) == 2 && cache.is_contiguous(), who,
+              ": kv_cache must be a contiguous [2, num_blocks, block_size, ..., row words]");
+  int64_t words = 1;
+  for (int64_t d = 3; d < cache.dim(); ++d) words *= cache.size(d);
+  const int64_t want = lmcb_kv4_row_words(heads, head_size);
+  TORCH_CHECK(want > 0, who, ": head_size must be a multiple of 8, at most 256, got ", head_size);
+  TORCH_CHECK(words == want, who, ": kv_cache rows have ", words, " words, ", heads,
+              " heads of ", head_size, " need ", want);
+}
+
+}  // namespace
+
+void build_slot_mapping(const torch::Tensor& context_lens, const torch::Tensor& query_lens,
+                        torch::Tensor& block_table, const torch::Tensor& free_blocks,
+                        int64_t block_size, torch::Tensor& slot_mapping, torch::Tensor& positions,
+                        torch::Tensor& query_start, torch::Tensor& seq_lens,
+                        torch::Tensor& blocks_used) {
+  const char* who = "build_slot_mapping";
+  TORCH_CHECK(block_table.is_cuda(), who, ": block_table must be a CUDA tensor");
+  const torch::Device dev = block_table.device();
+  TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt &&
+                  (block_table.size(1) <= 1 || block_table.stride(1) == 1) &&
+                  (block_table.size(0) <= 1 || block_table.stride(0) >= block_table.size(1)),
+              who, ": block_table must be int32 [num_requests, max_blocks] with dense rows");
+  const int64_t batch = block_table.size(0);
+  TORCH_CHECK(batch < (int64_t(1) << 31), who, ": too many requests");
+  check_index(context_lens, dev, who, "context_lens", batch, false);
+  check_index(query_lens, dev, who, "query_lens", batch, false);
+  TORCH_CHECK(context_lens.scalar_type() == query_lens.scalar_type(), who,
+              ": context_lens and query_lens must have the same dtype");
+  check_index(free_blocks, dev, who, "free_blocks", free_blocks.numel(), true);
+  check_index(slot_mapping, dev, who, "slot_mapping", slot_mapping.numel(), false);
+  check_index(positions, dev, who, "positions", slot_mapping.numel(), false);
+  TORCH_CHECK(slot_mapping.scalar_type() == positions.scalar_type(), who,
+              ": slot_mapping and positions must have the same dtype");
+  check_index(query_start, dev, who, "query_start", batch + 1, true);
+  check_index(seq_lens, dev, who, "seq_lens", batch, true);
+  check_index(blocks_used, dev, who, "blocks_used", 1, true);
+  TORCH_CHECK(block_size > 0 && block_size < (int64_t(1) << 31), who,
+              ": block_size must be positive");
+  const torch::Tensor* outs[] = {&block_table, &slot_mapping, &positions,
+                                 &query_start, &seq_lens,     &blocks_used};
+  const torch::Tensor* ins[] = {&context_lens, &query_lens, &free_blocks};
+  for (size_t i = 0; i < 6; ++i) {
+    for (size_t j = i + 1; j < 6; ++j) {
+      TORCH_CHECK(!overlap(*outs[i], *outs[j]), who, ": outputs overlap");
+    }
+    for (const torch::Tensor* in : ins) {
+      TORCH_CHECK(!overlap(*outs[i], *in), who, ": an output overlaps an input");
+    }
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  check_status(lmcb_build_slot_mapping(
+      context_lens.data_ptr(), query_lens.data_ptr(), to_slot_dtype(context_lens.scalar_type()),
+      static_cast<int32_t>(batch), static_cast<int32_t*>(block_table.data_ptr()),
+      batch > 1 ? block_table.stride(0) : block_table.size(1),
+      static_cast<int32_t>(std::min<int64_t>(block_table.size(1), INT32_MAX)),
+      static_cast<const int32_t*>(free_blocks.data_ptr()), free_blocks.numel(),
+      static_cast<int32_t>(block_size), slot_mapping.numel(), slot_mapping.data_ptr(),
+      positions.data_ptr(), to_slot_dtype(slot_mapping.scalar_type()),
+      static_cast<int32_t*>(query_start.data_ptr()), static_cast<int32_t*>(seq_lens.data_ptr()),
+      static_cast<int32_t*>(blocks_used.data_ptr()), current_stream()));
+}
+
+void qk_norm_rope(const torch::Tensor& query, const torch::Tensor& key,
+                  const c10::optional<torch::Tensor>& query_weight,
+                  const c10::optional<torch::Tensor>& key_weight, const torch::Tensor& positions,
+                  const torch::Tensor& cos_sin_cache, double eps, bool is_neox,
+                  torch::Tensor& query_out, torch::Tensor& key_out) {
+  const char* who = "qk_norm_rope";
+  TORCH_CHECK(query.is_cuda(), who, ": query must be a CUDA tensor");
+  const torch::Device dev = query.device();
+  check_heads(query, dev, who, "query");
+  check_heads(key, dev, who, "key");
+  check_heads(query_out, dev, who, "query_out");
+  check_heads(key_out, dev, who, "key_out");
+  const int64_t tokens = query.size(0), head_size = query.size(2);
+  TORCH_CHECK(key.size(0) == tokens && key.size(2) == head_size, who,
+              ": query and key must have the same tokens and head size");
+  TORCH_CHECK(query_out.sizes() == query.sizes() && key_out.sizes() == key.sizes(), who,
+              ": outputs must have their inputs' shapes");
+  TORCH_CHECK(key.scalar_type() == query.scalar_type() &&
+                  query_out.scalar_type() == query.scalar_type() &&
+                  key_out.scalar_type() == query.scalar_type(),
+              who, ": query, key and outputs must have the same dtype");
+  check_index(positions, dev, who, "positions", tokens, false);
+  check_cuda(cos_sin_cache, dev, who, "cos_sin_cache");
+  TORCH_CHECK(cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous(), who,
+              ": cos_sin_cache must be a contiguous [max_position, rot_dim] tensor");
+  const void* weights[2] = {nullptr, nullptr};
+  int weight_types[2] = {LMCB_DTYPE_FP32, LMCB_DTYPE_FP32};
+  const c10::optional<torch::Tensor>* given[2] = {&query_weight, &key_weight};
+  for (int i = 0; i < 2; ++i) {
+    if (!given[i]->has_value()) continue;
+    const torch::Tensor& w = given[i]->value();
+    check_cuda(w, dev, who, i == 0 ? "query_weight" : "key_weight");
+    TORCH_CHECK(w.dim() == 1 && w.is_contiguous() && w.size(0) == head_size, who,
+                ": a weight must be a contiguous vector of head_size entries");
+    weights[i] = w.data_ptr();
+    weight_types[i] = to_lmcb_dtype(w.scalar_type());
+  }
+  // An output is its input, element for element, or shares nothing with
+  // either input (two parts of one packed projection both count).
+  const auto in_place = [](const torch::Tensor& out, const torch::Tensor& in) {
+    return out.data_ptr() == in.data_ptr() && token_stride(out) == token_stride(in);
+  };
+  const bool q_in_place = in_place(query_out, query), k_in_place = in_place(key_out, key);
+  TORCH_CHECK(q_in_place || (!overlap(query_out, query) && !overlap(query_out, key)), who,
+              ": query_out must be query or overlap no input");
+  TORCH_CHECK(k_in_place || (!overlap(key_out, key) && !overlap(key_out, query)), who,
+              ": key_out must be key or overlap no input");
+  TORCH_CHECK((q_in_place && k_in_place) || !overlap(query_out, key_out), who,
+              ": outputs overlap");
+  const c10::cuda::CUDAGuard guard(dev);
+  check_status(lmcb_qk_norm_rope(
+      query.data_ptr(), key.data_ptr(), to_lmcb_dtype(query.scalar_type()), token_stride(query),
+      token_stride(key), weights[0], weight_types[0], weights[1], weight_types[1],
+      positions.data_ptr(), to_slot_dtype(positions.scalar_type()), cos_sin_cache.data_ptr(),
+      to_lmcb_dtype(cos_sin_cache.scalar_type()), cos_sin_cache.size(1), cos_sin_cache.size(0),
+      is_neox ? 1 : 0, eps, tokens, query.size(1), key.size(1), head_size, query_out.data_ptr(),
+      token_stride(query_out), key_out.data_ptr(), token_stride(key_out), current_stream()));
+}
+
+int64_t kv4_row_words(int64_t num_heads, int64_t head_size) {
+  const int64_t words = lmcb_kv4_row_words(num_heads, head_size);
+  TORCH_CHECK(words > 0, "kv4_row_words: num_heads must be positive and head_size a multiple of 8, "
+                         "at most 256");
+  return words;
+}
+
+namespace {
+
+void check_kv4_rows(const torch::Tensor& key, const torch::Tensor& value,
+                    const torch::Tensor& kv_cache, const torch::Tensor& slot_mapping,
+                    const char* who) {
+  TORCH_CHECK(kv_cache.is_cuda(), who, ": kv_cache must be a CUDA tensor");
+  const torch::Device dev = kv_cache.device();
+  check_heads(key, dev, who, "key");
+  check_heads(value, dev, who, "value");
+  TORCH_CHECK(key.sizes() == value.sizes() && key.scalar_type() == value.scalar_type(), who,
+              ": key and value must have the same shape and dtype");
+  check_kv4_cache(kv_cache, dev, who, key.size(1), key.size(2));
+  check_index(slot_mapping, dev, who, "slot_mapping", key.size(0), false);
+}
+
+}  // namespace
+
+void kv4_store(const torch::Tensor& key, const torch::Tensor& value, torch::Tensor& kv_cache,
+               const torch::Tensor& slot_mapping) {
+  check_kv4_rows(key, value, kv_cache, slot_mapping, "kv4_store");
+  const c10::cuda::CUDAGuard guard(kv_cache.device());
+  check_status(lmcb_kv4_store(
+      key.data_ptr(), value.data_ptr(), to_lmcb_dtype(key.scalar_type()), token_stride(key),
+      token_stride(value), static_cast<int32_t*>(kv_cache.data_ptr()), kv_cache.size(1),
+      kv_cache.size(2), slot_mapping.data_ptr(), to_slot_dtype(slot_mapping.scalar_type()),
+      key.size(0), key.size(1), key.size(2), current_stream()));
+}
+
+void kv4_load(const torch::Tensor& kv_cache, const torch::Tensor& slot_mapping, torch::Tensor& key,
+              torch::Tensor& value) {
+  check_kv4_rows(key, value, kv_cache, slot_mapping, "kv4_load");
+  TORCH_CHECK(!overlap(key, value), "kv4_load: key and value overlap");
+  const c10::cuda::CUDAGuard guard(kv_cache.device());
+  check_status(lmcb_kv4_load(
+      static_cast<const int32_t*>(kv_cache.data_ptr()), kv_cache.size(1), kv_cache.size(2),
+      slot_mapping.data_ptr(), to_slot_dtype(slot_mapping.scalar_type()), key.data_ptr(),
+      value.data_ptr(), to_lmcb_dtype(key.scalar_type()), token_stride(key), token_stride(value),
+      key.size(0), key.size(1), key.size(2), current_stream()));
+}
+
+void kv4_attention(const torch::Tensor& query, const torch::Tensor& kv_cache,
+                   const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                   const c10::optional<torch::Tensor>& query_start, int64_t max_query_len,
+                   int64_t max_seq_len, int64_t num_kv_heads, double scale, int64_t window,
+                   int64_t sinks, torch::Tensor& out) {
+  const char* who = "kv4_attention";
+  TORCH_CHECK(query.is_cuda(), who, ": query must be a CUDA tensor");
+  const torch::Device dev = query.device();
+  check_heads(query, dev, who, "query");
+  check_heads(out, dev, who, "out");
+  TORCH_CHECK(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type(), who,
+              ": out must have the query's shape and dtype");
+  TORCH_CHECK(num_kv_heads > 0 && query.size(1) % num_kv_heads == 0, who,
+              ": num_kv_heads must divide the query heads");
+  check_kv4_cache(kv_cache, dev, who, num_kv_heads, query.size(2));
+  check_cuda(block_table, dev, who, "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt &&
+                  (block_table.size(1) <= 1 || block_table.stride(1) == 1) &&
+                  (block_table.size(0) <= 1 || block_table.stride(0) >= block_table.size(1)),
+              who, ": block_table must be int32 [batch, max_blocks] with dense rows");
+  const int64_t batch = block_table.size(0);
+  check_index(seq_lens, dev, who, "seq_lens", batch, true);
+  const int32_t* starts = nullptr;
+  if (query_start.has_value()) {
+    check_index(*query_start, dev, who, "query_start", batch + 1, true);
+    starts = static_cast<const int32_t*>(query_start->data_ptr());
+  } else {
+    TORCH_CHECK(query.size(0) >= batch, who, ": without query_start every request has one query");
+  }
+  TORCH_CHECK(!overlap(out, query) && !overlap(out, kv_cache), who, ": out overlaps an input");
+  const c10::cuda::CUDAGuard guard(dev);
+  size_t bytes = 0;
+  check_status(lmcb_kv4_attention_workspace(batch, max_query_len, max_seq_len, num_kv_heads,
+                                            query.size(1), query.size(2), window, sinks, &bytes));
+  torch::Tensor workspace;
+  if (bytes > 0) {
+    workspace = torch::empty({static_cast<int64_t>(bytes)},
+                             torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+  }
+  check_status(lmcb_kv4_attention(
+      query.data_ptr(), to_lmcb_dtype(query.scalar_type()), token_stride(query), query.size(0),
+      static_cast<const int32_t*>(kv_cache.data_ptr()), kv_cache.size(1), kv_cache.size(2),
+      static_cast<const int32_t*>(block_table.data_ptr()),
+      batch > 1 ? block_table.stride(0) : block_table.size(1), block_table.size(1),
+      static_cast<const int32_t*>(seq_lens.data_ptr()), starts, batch, max_query_len, max_seq_len,
+      num_kv_heads, query.size(1), query.size(2), scale, window, sinks, out.data_ptr(),
+      token_stride(out), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, current_stream()));
+}
+
 uint32_t device_status(int device) {
   uint32_t flags = 0;
   check_status(lmcb_device_status(device, &flags));
@@ -696,6 +974,12 @@ PYBIND11_MODULE(c_ops, m) {
   // Additions beyond the reference surface.
   m.def("multi_layer_kv_transfer_batched", &multi_layer_kv_transfer_batched);
   m.def("single_layer_kv_transfer_batched", &single_layer_kv_transfer_batched);
+  m.def("build_slot_mapping", &build_slot_mapping);
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("kv4_row_words", &kv4_row_words);
+  m.def("kv4_store", &kv4_store);
+  m.def("kv4_load", &kv4_load);
+  m.def("kv4_attention", &kv4_attention);
   m.def("host_unregister", &unregister_memory);
   m.def("get_device_ptr", &get_device_ptr);
   m.def("device_status", &device_status);

@@ -400,6 +400,349 @@ bool float_type(int t) {
   return t == LMCB_DTYPE_FP32 || t == LMCB_DTYPE_BF16 || t == LMCB_DTYPE_FP16;
 }
 
+
+// ---------------------------------------------------------------------------
+// Per-head norm of queries and keys with the rotation in the same pass
+// (qk_norm_rope)
+// ---------------------------------------------------------------------------
+//
+// Every head row x of D values becomes
+//   y = x / sqrt(mean(x^2) + eps) * w,
+// and its first rot_dim values are rotated by the angles of the token's
+// position: y1' = y1 cos - y2 sin, y2' = y2 cos + y1 sin, in the pairs of the
+// rotary layouts above. Squares, sum, scale and rotation are fp32; the result
+// is rounded once to the row's type, where a norm and a rotation run one after
+// the other round twice.
+
+struct QkNormParams {
+  const void* in[2];   // q, k
+  void* out[2];
+  const void* weight[2];  // NULL: no weight
+  int weight_type[2];
+  int64_t in_stride[2];  // elements between tokens
+  int64_t out_stride[2];
+  const void* positions;
+  int pos64;
+  const void* cache;
+  int cache_type;
+  int64_t num_tokens;
+  int32_t heads[2];
+  int32_t head_size;
+  int32_t rot_dim;
+  int64_t max_position;
+  float eps;
+  unsigned int* status;
+};
+
+// N consecutive values of a tensor whose type is known at run time only (the
+// weights and the cos/sin rows: once per row or token, the branch is uniform).
+template <int N>
+__device__ __forceinline__ void load_run_typed(const void* base, int type, int64_t at,
+                                               float (&out)[N]) {
+  if (type == LMCB_DTYPE_FP32) {
+    load_cache_run<float, N>(static_cast<const float*>(base) + at, out);
+  } else if (type == LMCB_DTYPE_BF16) {
+    load_cache_run<__nv_bfloat16, N>(static_cast<const __nv_bfloat16*>(base) + at, out);
+  } else {
+    load_cache_run<__half, N>(static_cast<const __half*>(base) + at, out);
+  }
+}
+
+__device__ __forceinline__ float load_typed(const void* base, int type, int64_t at) {
+  if (type == LMCB_DTYPE_FP32) return static_cast<const float*>(base)[at];
+  if (type == LMCB_DTYPE_BF16) return to_f(static_cast<const __nv_bfloat16*>(base)[at]);
+  return to_f(static_cast<const __half*>(base)[at]);
+}
+
+__device__ __forceinline__ int64_t qk_position(const QkNormParams& p, int64_t token) {
+  return p.pos64 ? static_cast<const int64_t*>(p.positions)[token]
+                 : static_cast<int64_t>(static_cast<const int32_t*>(p.positions)[token]);
+}
+
+constexpr int kQkThreads = 256;
+constexpr int kQkRowsInFlight = 2;
+
+// kLanes lanes share a head row; a lane holds two 16-byte vectors of it: for
+// neox a vector of the first rotary half and its partner in the second (so a
+// pair never leaves its lane), else two vectors of adjacent pairs; lanes behind
+// the rotated part hold two vectors of the rest. A warp takes one token and a
+// run of its heads (q heads, then k heads), 32 / kLanes heads a pass: the
+// cos/sin values a lane needs are the same for every head, so it loads them
+// once for the run.
+template <typename T, bool kNeox, int kLanes>
+__global__ void __launch_bounds__(kQkThreads)
+qk_norm_rope_vec_kernel(const QkNormParams p, const uint32_t num_items, const FastDiv div_runs,
+                        const int heads_per_run) {
+  constexpr int E = 16 / sizeof(T);
+  constexpr int kHeadsPerPass = 32 / kLanes;
+  using V = Vec16<T>;
+  const int lane = threadIdx.x % 32;
+  const int l = lane % kLanes;
+  const int sub = lane / kLanes;
+  const int D = p.head_size, rot = p.rot_dim;
+  const bool active = l * 2 * E < D;
+  // the two vectors of this lane, and whether they are rotated
+  int e0, e1;
+  bool turn0, turn1;
+  if constexpr (kNeox) {
+    const int pairs = rot / 2 / E;  // lanes that hold rotated vectors
+    turn0 = turn1 = l < pairs;
+    e0 = l < pairs ? l * E : rot + (l - pairs) * 2 * E;
+    e1 = l < pairs ? rot / 2 + l * E : e0 + E;
+  } else {
+    e0 = l * 2 * E;
+    e1 = e0 + E;
+    turn0 = e0 < rot;
+    turn1 = e1 < rot;
+  }
+  const int all_heads = p.heads[0] + p.heads[1];
+  const uint32_t warps = gridDim.x * (kQkThreads / 32);
+  for (uint32_t item = blockIdx.x * (kQkThreads / 32) + threadIdx.x / 32; item < num_items;
+       item += warps) {
+    const uint32_t t = div_runs.div(item);
+    const int h_first = static_cast<int>(item - t * div_runs.d) * heads_per_run;
+    const int h_last = min(h_first + heads_per_run, all_heads);
+    const int64_t pos = qk_position(p, t);
+    float cs[E], sn[E];  // neox: one run of E; else E / 2 for each vector
+    for (int h0 = h_first; h0 < h_last; h0 += kHeadsPerPass * kQkRowsInFlight) {
+      V x[kQkRowsInFlight][2];
+#pragma unroll
+      for (int u = 0; u < kQkRowsInFlight; ++u) {
+        const int h = h0 + u * kHeadsPerPass + sub;
+        if (h < h_last && active) {
+          const int which = h >= p.heads[0];
+          const T* row = static_cast<const T*>(p.in[which]) +
+                         static_cast<int64_t>(t) * p.in_stride[which] +
+                         static_cast<int64_t>(h - (which ? p.heads[0] : 0)) * D;
+          x[u][0] = *reinterpret_cast<const V*>(row + e0);
+          x[u][1] = *reinterpret_cast<const V*>(row + e1);
+        }
+      }
+      if (h0 == h_first) {
+        if (pos < 0 || pos >= p.max_position) {
+          if (lane == 0 && h_first == 0) {
+            raise_flag(p.status, LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE);
+          }
+          break;  // uniform: the token's rows are left as they were
+        }
+        const int64_t row = pos * rot;
+        if (kNeox) {
+          if (active && turn0) {
+            load_run_typed<E>(p.cache, p.cache_type, row + e0, cs);
+            load_run_typed<E>(p.cache, p.cache_type, row + rot / 2 + e0, sn);
+          }
+        } else {
+          float c2[E / 2], s2[E / 2];
+          if (active && turn0) {
+            load_run_typed<E / 2>(p.cache, p.cache_type, row + e0 / 2, c2);
+            load_run_typed<E / 2>(p.cache, p.cache_type, row + rot / 2 + e0 / 2, s2);
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) cs[j] = c2[j], sn[j] = s2[j];
+          }
+          if (active && turn1) {
+            load_run_typed<E / 2>(p.cache, p.cache_type, row + e1 / 2, c2);
+            load_run_typed<E / 2>(p.cache, p.cache_type, row + rot / 2 + e1 / 2, s2);
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) cs[E / 2 + j] = c2[j], sn[E / 2 + j] = s2[j];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kQkRowsInFlight; ++u) {
+        const int h = h0 + u * kHeadsPerPass + sub;
+        const bool live = h < h_last && active;
+        const int which = h >= p.heads[0];
+        float a[E], b[E];
+        float ss = 0.0f;
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            a[j] = to_f(x[u][0].v[j]);
+            b[j] = to_f(x[u][1].v[j]);
+            ss = fmaf(a[j], a[j], ss);
+            ss = fmaf(b[j], b[j], ss);
+          }
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!live) continue;
+        const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+        if (p.weight[which] != nullptr) {
+          float wa[E], wb[E];
+          load_run_typed<E>(p.weight[which], p.weight_type[which], e0, wa);
+          load_run_typed<E>(p.weight[which], p.weight_type[which], e1, wb);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            a[j] = a[j] * inv * wa[j];
+            b[j] = b[j] * inv * wb[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            a[j] *= inv;
+            b[j] *= inv;
+          }
+        }
+        if constexpr (kNeox) {
+          if (turn0) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              float y1, y2;
+              rotate_pair(a[j], b[j], cs[j], sn[j], y1, y2);
+              a[j] = y1;
+              b[j] = y2;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j) {
+            float y1, y2;
+            if (turn0) {
+              rotate_pair(a[2 * j], a[2 * j + 1], cs[j], sn[j], y1, y2);
+              a[2 * j] = y1;
+              a[2 * j + 1] = y2;
+            }
+            if (turn1) {
+              rotate_pair(b[2 * j], b[2 * j + 1], cs[E / 2 + j], sn[E / 2 + j], y1, y2);
+              b[2 * j] = y1;
+              b[2 * j + 1] = y2;
+            }
+          }
+        }
+        T* row = static_cast<T*>(p.out[which]) + static_cast<int64_t>(t) * p.out_stride[which] +
+                 static_cast<int64_t>(h - (which ? p.heads[0] : 0)) * D;
+        V ya, yb;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          ya.v[j] = from_f<T>(a[j]);
+          yb.v[j] = from_f<T>(b[j]);
+        }
+        *reinterpret_cast<V*>(row + e0) = ya;
+        *reinterpret_cast<V*>(row + e1) = yb;
+      }
+    }
+  }
+}
+
+// The same for every other size and alignment: a warp a head row, element by
+// element. The second pass reads and writes an element in one lane only, so
+// the output may be the input.
+template <typename T>
+__global__ void __launch_bounds__(kQkThreads)
+qk_norm_rope_kernel(const QkNormParams p, const int is_neox, const FastDiv div_heads,
+                    const uint32_t num_rows) {
+  const int lane = threadIdx.x % 32;
+  const int D = p.head_size, rot = p.rot_dim, half = rot / 2;
+  for (uint32_t row = blockIdx.x * (kQkThreads / 32) + threadIdx.x / 32; row < num_rows;
+       row += gridDim.x * (kQkThreads / 32)) {
+    const uint32_t t = div_heads.div(row);
+    const int h = static_cast<int>(row - t * div_heads.d);
+    const int which = h >= p.heads[0];
+    const int64_t head = h - (which ? p.heads[0] : 0);
+    const T* in = static_cast<const T*>(p.in[which]) + t * p.in_stride[which] + head * D;
+    T* out = static_cast<T*>(p.out[which]) + t * p.out_stride[which] + head * D;
+    const int64_t pos = qk_position(p, t);
+    if (pos < 0 || pos >= p.max_position) {
+      if (lane == 0) raise_flag(p.status, LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE);
+      continue;  // uniform across the warp
+    }
+    float ss = 0.0f;
+    for (int i = lane; i < D; i += 32) {
+      const float v = to_f(in[i]);
+      ss = fmaf(v, v, ss);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+    const void* w = p.weight[which];
+    const int wt = p.weight_type[which];
+    for (int i = lane; i < half; i += 32) {
+      const int i1 = is_neox ? i : 2 * i;
+      const int i2 = is_neox ? i + half : 2 * i + 1;
+      const float w1 = w == nullptr ? 1.0f : load_typed(w, wt, i1);
+      const float w2 = w == nullptr ? 1.0f : load_typed(w, wt, i2);
+      const float c = load_typed(p.cache, p.cache_type, pos * rot + i);
+      const float s = load_typed(p.cache, p.cache_type, pos * rot + half + i);
+      float y1, y2;
+      rotate_pair(to_f(in[i1]) * inv * w1, to_f(in[i2]) * inv * w2, c, s, y1, y2);
+      out[i1] = from_f<T>(y1);
+      out[i2] = from_f<T>(y2);
+    }
+    for (int i = rot + lane; i < D; i += 32) {
+      const float w1 = w == nullptr ? 1.0f : load_typed(w, wt, i);
+      out[i] = from_f<T>(to_f(in[i]) * inv * w1);
+    }
+  }
+}
+
+// True when every access of qk_norm_rope_vec_kernel is a whole aligned vector.
+template <typename T>
+bool qk_vec_ok(const QkNormParams& p, bool neox) {
+  constexpr int E = 16 / sizeof(T);
+  const auto aligned = [](const void* a) { return reinterpret_cast<uintptr_t>(a) % 16 == 0; };
+  for (int i = 0; i < 2; ++i) {
+    if (p.heads[i] == 0) continue;
+    if (!aligned(p.in[i]) || !aligned(p.out[i]) || p.in_stride[i] % E != 0 ||
+        p.out_stride[i] % E != 0 || (p.weight[i] != nullptr && !aligned(p.weight[i]))) {
+      return false;
+    }
+  }
+  if (!aligned(p.cache) || p.head_size % (2 * E) != 0 || p.head_size > 32 * 2 * E) return false;
+  // neox: whole vectors in each rotary half and whole vector pairs behind
+  // them; else whole vectors rotated. A cache row of any type starts on a
+  // vector of the widths read when rot_dim is a multiple of 16 (8 two-byte
+  // values, half of a row).
+  if (p.rot_dim % 16 != 0) return false;
+  return neox ? (p.head_size - p.rot_dim) % (2 * E) == 0 : p.rot_dim % E == 0;
+}
+
+template <typename T, bool kNeox, int kLanes>
+void launch_qk_vec(const QkNormParams& p, cudaStream_t stream) {
+  constexpr int kPerStep = 32 / kLanes * kQkRowsInFlight;
+  const int heads = p.heads[0] + p.heads[1];
+  // A warp's run of heads: as few as one step while that leaves warps idle,
+  // all of them once the tokens alone fill the GPU.
+  const int64_t slots = static_cast<int64_t>(current_sm_count()) * 24;
+  int64_t runs = (heads + kPerStep - 1) / kPerStep;
+  while (runs > 1 && p.num_tokens * (runs / 2) >= slots) runs /= 2;
+  int per_run = static_cast<int>((heads + runs - 1) / runs);
+  per_run = (per_run + kPerStep - 1) / kPerStep * kPerStep;
+  runs = (heads + per_run - 1) / per_run;
+  const int64_t items = p.num_tokens * runs;
+  const int64_t want = (items + kQkThreads / 32 - 1) / (kQkThreads / 32);
+  const int64_t most = static_cast<int64_t>(current_sm_count()) * 8;
+  qk_norm_rope_vec_kernel<T, kNeox, kLanes>
+      <<<static_cast<unsigned>(want < most ? want : most), kQkThreads, 0, stream>>>(
+          p, static_cast<uint32_t>(items), FastDiv(static_cast<uint32_t>(runs)), per_run);
+}
+
+template <typename T, bool kNeox>
+void launch_qk_lanes(const QkNormParams& p, cudaStream_t stream) {
+  constexpr int E = 16 / sizeof(T);
+  const int lanes = p.head_size / (2 * E);
+  if (lanes <= 4) launch_qk_vec<T, kNeox, 4>(p, stream);
+  else if (lanes <= 8) launch_qk_vec<T, kNeox, 8>(p, stream);
+  else if (lanes <= 16) launch_qk_vec<T, kNeox, 16>(p, stream);
+  else launch_qk_vec<T, kNeox, 32>(p, stream);
+}
+
+template <typename T>
+cudaError_t launch_qk(const QkNormParams& p, bool neox, cudaStream_t stream) {
+  if (qk_vec_ok<T>(p, neox)) {
+    if (neox) launch_qk_lanes<T, true>(p, stream);
+    else launch_qk_lanes<T, false>(p, stream);
+  } else {
+    const int heads = p.heads[0] + p.heads[1];
+    const int64_t rows = p.num_tokens * heads;
+    const int64_t want = (rows + kQkThreads / 32 - 1) / (kQkThreads / 32);
+    const int64_t most = static_cast<int64_t>(current_sm_count()) * 8;
+    qk_norm_rope_kernel<T><<<static_cast<unsigned>(want < most ? want : most), kQkThreads, 0,
+                             stream>>>(p, neox ? 1 : 0, FastDiv(static_cast<uint32_t>(heads)),
+                                       static_cast<uint32_t>(rows));
+  }
+  return cudaGetLastError();
+}
+
 }  // namespace
 }  // namespace lmcb
 
@@ -455,6 +798,78 @@ int lmcb_rotary_embedding_k_fused(const void* oldPositions, const void* newPosit
     default: err = lmcb::launch_rope_cache<__half>(p, cacheType, posType, s); break;
   }
   if (err != cudaSuccess) return lmcb::cuda_fail(err, who);
+  return LMCB_OK;
+}
+
+int lmcb_qk_norm_rope(const void* query, const void* key, int type, int64_t queryTokenStride,
+                      int64_t keyTokenStride, const void* queryWeight, int queryWeightType,
+                      const void* keyWeight, int keyWeightType, const void* positions, int posType,
+                      const void* cosSinCache, int cacheType, int64_t rotDim, int64_t maxPosition,
+                      int isNeox, double eps, int64_t numTokens, int64_t numQueryHeads,
+                      int64_t numKeyHeads, int64_t headSize, void* queryOut,
+                      int64_t queryOutStride, void* keyOut, int64_t keyOutStride, void* stream) {
+  lmcb::clear_error();
+  const std::string who = "qk_norm_rope";
+  if (!lmcb::float_type(type) || !lmcb::float_type(cacheType) ||
+      (queryWeight != nullptr && !lmcb::float_type(queryWeightType)) ||
+      (keyWeight != nullptr && !lmcb::float_type(keyWeightType))) {
+    return lmcb::fail(LMCB_ERR_UNSUPPORTED_DTYPE, who + ": ScalarType not supported.");
+  }
+  if (posType != LMCB_DTYPE_INT64 && posType != LMCB_DTYPE_INT32) {
+    return lmcb::fail(LMCB_ERR_UNSUPPORTED_DTYPE, who + ": positions must be int64 or int32.");
+  }
+  if (numTokens < 0 || numQueryHeads < 0 || numKeyHeads < 0 || headSize <= 0 ||
+      headSize > 65536 || rotDim < 0 || rotDim % 2 != 0 || rotDim > headSize ||
+      maxPosition <= 0 || numQueryHeads > 65536 || numKeyHeads > 65536 ||
+      queryTokenStride < numQueryHeads * headSize || queryOutStride < numQueryHeads * headSize ||
+      keyTokenStride < numKeyHeads * headSize || keyOutStride < numKeyHeads * headSize) {
+    return lmcb::fail(LMCB_ERR_INVALID_ARGUMENT,
+                      who + ": invalid shape (rot_dim must be even and <= head_size).");
+  }
+  const int64_t heads = numQueryHeads + numKeyHeads;
+  if (numTokens == 0 || heads == 0) return LMCB_OK;
+  if (numTokens > 0x7fffffff / heads) {
+    return lmcb::fail(LMCB_ERR_INVALID_ARGUMENT, who + ": too many head rows in one call.");
+  }
+  if ((numQueryHeads > 0 && (query == nullptr || queryOut == nullptr)) ||
+      (numKeyHeads > 0 && (key == nullptr || keyOut == nullptr)) || positions == nullptr ||
+      (rotDim > 0 && cosSinCache == nullptr)) {
+    return lmcb::fail(LMCB_ERR_INVALID_ARGUMENT, who + ": NULL pointer.");
+  }
+  lmcb::QkNormParams p;
+  p.in[0] = query;
+  p.in[1] = key;
+  p.out[0] = queryOut;
+  p.out[1] = keyOut;
+  p.weight[0] = queryWeight;
+  p.weight[1] = keyWeight;
+  p.weight_type[0] = queryWeightType;
+  p.weight_type[1] = keyWeightType;
+  p.in_stride[0] = queryTokenStride;
+  p.in_stride[1] = keyTokenStride;
+  p.out_stride[0] = queryOutStride;
+  p.out_stride[1] = keyOutStride;
+  p.positions = positions;
+  p.pos64 = posType == LMCB_DTYPE_INT64;
+  p.cache = cosSinCache;
+  p.cache_type = cacheType;
+  p.num_tokens = numTokens;
+  p.heads[0] = static_cast<int32_t>(numQueryHeads);
+  p.heads[1] = static_cast<int32_t>(numKeyHeads);
+  p.head_size = static_cast<int32_t>(headSize);
+  p.rot_dim = static_cast<int32_t>(rotDim);
+  p.max_position = maxPosition;
+  p.eps = static_cast<float>(eps);
+  p.status = lmcb::device_status_ptr();
+  if (p.status == nullptr) return LMCB_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err;
+  switch (type) {
+    case LMCB_DTYPE_FP32: err = lmcb::launch_qk<float>(p, isNeox != 0, s); break;
+    case LMCB_DTYPE_BF16: err = lmcb::launch_qk<__nv_bfloat16>(p, isNeox != 0, s); break;
+    default: err = lmcb::launch_qk<__half>(p, isNeox != 0, s); break;
+  }
+  if (err != cudaSuccess) return lmcb::cuda_fail(err, who.c_str());
   return LMCB_OK;
 }
 

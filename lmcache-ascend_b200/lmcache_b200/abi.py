@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import c_char_p, c_double, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "liblmcache_b200.so")
 
@@ -36,6 +36,8 @@ LMCB_DEVICE_FLAG_SYMBOL_OUT_OF_RANGE = 0x2
 LMCB_DEVICE_FLAG_STREAM_OVERFLOW = 0x4
 LMCB_DEVICE_FLAG_WAIT_TIMEOUT = 0x8
 LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE = 0x10
+LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE = 0x20
+LMCB_DEVICE_FLAG_PAGES_EXHAUSTED = 0x40
 
 LMCB_NOALLOC_STAGING_BYTES = 64 << 20
 
@@ -117,6 +119,39 @@ SIGNATURES: dict[str, tuple] = {
         c_int,
         [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
          c_void_p, c_int, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "lmcb_build_slot_mapping": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int64,
+         c_int32, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "lmcb_qk_norm_rope": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p,
+         c_int, c_void_p, c_int, c_int64, c_int64, c_int, c_double, c_int64, c_int64, c_int64,
+         c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "lmcb_kv4_row_words": (c_int64, [c_int64, c_int64]),
+    "lmcb_kv4_store": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int,
+         c_int64, c_int64, c_int64, c_void_p],
+    ),
+    "lmcb_kv4_load": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64,
+         c_int64, c_int64, c_int64, c_void_p],
+    ),
+    "lmcb_kv4_attention": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+         c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_double, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p],
+    ),
+    "lmcb_kv4_attention_workspace": (
+        c_int,
+        [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         ctypes.POINTER(c_size_t)],
     ),
 }
 
