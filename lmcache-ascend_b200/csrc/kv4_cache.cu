@@ -8,14 +8,12 @@
 // row's 4 bytes are then 1/17 of its 68 (D = 128). NaN counts as 0 and values
 // beyond the fp16 range as its ends, so that every row is finite.
 //
-// The code is the exact one: (x - z) * (1 / s) in fp32 is off by less than
-// 2^-17 for quotients up to 17, and a lane whose quotient lies that close to a
-// border between two codes repeats it in 64 bits. So the codes depend on no
-// rounding of the reciprocal and equal those of any exact computation.
+// The code is the exact one, see word_of: it depends on no rounding of a
+// reciprocal and equals that of any exact computation.
 //
 // Both kernels are byte movers (2 D bytes of bf16 against D / 2 + 4): D / 8
 // lanes share a head row, a lane holds the eight values of one word (one
-// 16-byte access of a 16-bit type), and a lane has kRows rows in flight.
+// 16-byte access of a 16-bit type), and a lane has up to kMost rows in flight.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -32,7 +30,7 @@ namespace lmcb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;  // head rows in flight per lane
+constexpr int kMost = 4;  // head rows in flight per lane
 
 struct Kv4Params {
   const void* src[2];       // store: key, value rows
@@ -47,8 +45,8 @@ struct Kv4Params {
   int32_t num_tokens;
   int32_t num_heads;
   int32_t head_size;
-  uint32_t rows_per_half;  // num_tokens * num_heads
-  FastDiv div_heads;
+  uint32_t items_per_half;  // items of a group of lanes in K, or in V
+  FastDiv div_items;        // by items per token
   unsigned int* status;
 };
 
@@ -111,33 +109,84 @@ __device__ __forceinline__ float finite_half_range(float x) {
   return fminf(fmaxf(x, -65504.0f), 65504.0f);
 }
 
-// clamp(rne((x - z) / s), 0, 15), exact. `inv` is 1 / s rounded.
-__device__ __forceinline__ uint32_t code_of(float x, float z, float s, float inv) {
-  const float q = (x - z) * inv;
-  const float r = rintf(q);
-  if (fabsf(fabsf(q - r) - 0.5f) < 1.0f / 65536.0f) {
-    const double exact = (static_cast<double>(x) - static_cast<double>(z)) / static_cast<double>(s);
-    return static_cast<uint32_t>(fmin(fmax(rint(exact), 0.0), 15.0));
+// Smallest and largest of a head row over the lanes that share it, both NaN
+// where the row holds one. 16-bit types compare two values an instruction,
+// and (min, -max) is one register on its way through the lanes.
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair<__half> { using type = __half2; };
+
+template <typename T, int kGroup>
+__device__ __forceinline__ void row_range(const Eight<T>& x, bool active, float& lo, float& hi) {
+  if constexpr (sizeof(T) == 2) {
+    using P = typename Pair<T>::type;
+    const P* v = reinterpret_cast<const P*>(&x);
+    const P small = __hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3]));
+    const P large = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+    P both;
+    both.x = __hmin_nan(small.x, small.y);
+    both.y = __hneg(__hmax_nan(large.x, large.y));
+    if (!active) both.x = both.y = from_float<T>(INFINITY);
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) {
+      both = __hmin2_nan(both, __shfl_xor_sync(0xffffffffu, both, o));
+    }
+    lo = to_float(both.x);
+    hi = -to_float(both.y);
+  } else {
+    lo = INFINITY;
+    hi = -INFINITY;
+    bool nan = false;
+    if (active) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        nan = nan || x.v[i] != x.v[i];
+        lo = fminf(lo, x.v[i]);
+        hi = fmaxf(hi, x.v[i]);
+      }
+    }
+    if (nan) hi = INFINITY;  // out of range all the same
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
   }
-  return static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f));
 }
 
-// A row of the work list: rows are numbered half-major (K, then V), then by
-// token, then by head, so consecutive rows are consecutive in memory on the
-// 16/32-bit side.
-struct RowRef {
-  int half;
-  uint32_t token;
-  uint32_t head;
-};
+// One word of codes clamp(rne((x - z) / s), 0, 15) in 64 bits.
+__device__ __noinline__ uint32_t exact_word(const float (&v)[8], float z, float s) {
+  uint32_t word = 0;
+  for (int i = 0; i < 8; ++i) {
+    const double q = (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
+    word |= static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0)) << (4 * i);
+  }
+  return word;
+}
 
-__device__ __forceinline__ RowRef row_ref(const Kv4Params& p, uint32_t row) {
-  RowRef r;
-  r.half = row >= p.rows_per_half;
-  const uint32_t in_half = r.half ? row - p.rows_per_half : row;
-  r.token = p.div_heads.div(in_half);
-  r.head = in_half - r.token * p.div_heads.d;
-  return r;
+// The same in fp32: q is off by less than 2^-17 (a rounded difference, an
+// approximate reciprocal of 1 ulp and a rounded product, each 2^-23 of at most
+// 16 + 2^-6 before the clamp), so only a q that close to a border between two
+// codes needs more. Adding 1.5 2^23 rounds q to an integer, ties to even, in
+// the sum's low bits; a multiply-add by 16^i puts it in its place, and what the
+// eight exponent fields add up to is one constant.
+__device__ __forceinline__ uint32_t word_of(const float (&v)[8], float z, float s) {
+  constexpr float kMagic = 12582912.0f;
+  constexpr uint32_t kBias = 0x4B400000u * 0x11111111u;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  uint32_t word = 0;
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = fminf(fmaxf((v[i] - z) * inv, 0.0f), 15.0f);
+    const float r = q + kMagic;
+    off = fmaxf(off, fabsf(q - (r - kMagic)));
+    word += __float_as_uint(r) << (4 * i);
+  }
+  word -= kBias;
+  if (off > 0.5f - 1.0f / 65536.0f) word = exact_word(v, z, s);
+  return word;
 }
 
 __device__ __forceinline__ int64_t slot_of(const Kv4Params& p, uint32_t token) {
@@ -145,140 +194,166 @@ __device__ __forceinline__ int64_t slot_of(const Kv4Params& p, uint32_t token) {
                   : static_cast<int64_t>(static_cast<const int32_t*>(p.slots)[token]);
 }
 
+// What a group of lanes takes at once: kHeads consecutive heads of one token's
+// K or V row. Items are numbered half-major, then by token, so consecutive
+// groups read consecutive memory, and the slot and all addresses are found
+// once for kHeads head rows.
+struct Item {
+  int half;
+  uint32_t token;
+  int32_t head;   // the first one
+  int32_t count;  // heads of it, 0: nothing to do
+  int64_t slot;
+};
+
+template <int kHeads>
+__device__ __forceinline__ Item item_of(const Kv4Params& p, uint64_t at, bool flag) {
+  Item it;
+  it.count = 0;
+  if (at >= 2ull * p.items_per_half) return it;
+  it.half = at >= p.items_per_half;
+  const uint32_t in_half = static_cast<uint32_t>(at) - (it.half ? p.items_per_half : 0);
+  it.token = p.div_items.div(in_half);
+  it.head = static_cast<int32_t>(in_half - it.token * p.div_items.d) * kHeads;
+  it.slot = slot_of(p, it.token);
+  if (it.slot >= p.num_rows) {
+    if (flag) raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
+    it.slot = -1;
+  }
+  if (it.slot >= 0) it.count = min(kHeads, p.num_heads - it.head);
+  return it;
+}
+
 // kGroup lanes share a head row (D <= 8 * kGroup).
-template <typename T, int kGroup, bool kVec>
+template <typename T, int kGroup, int kHeads, bool kVec>
 __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Params p) {
   const int lane = threadIdx.x % kGroup;
-  const bool active = lane * 8 < p.head_size;
-  const uint32_t total = 2 * p.rows_per_half;
+  const int D = p.head_size;
+  const bool active = lane * 8 < D;
   constexpr uint32_t kGroups = kThreads / kGroup;
-  const int words = p.head_size / 8;
-  for (uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * (kGroups * kRows) + threadIdx.x / kGroup;
-       r0 - threadIdx.x / kGroup < total; r0 += static_cast<uint64_t>(gridDim.x) * kGroups * kRows) {
-    Eight<T> x[kRows];
-    int64_t slot[kRows];
-    RowRef ref[kRows];
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kGroups; base < 2ull * p.items_per_half;
+       base += static_cast<uint64_t>(gridDim.x) * kGroups) {
+    const Item it = item_of<kHeads>(p, base + threadIdx.x / kGroup, lane == 0);
+    Eight<T> x[kHeads] = {};
+    if (it.count > 0 && active) {
+      const T* src = static_cast<const T*>(it.half ? p.src[1] : p.src[0]) +
+                     static_cast<int64_t>(it.token) * (it.half ? p.token_stride[1] : p.token_stride[0]) +
+                     static_cast<int64_t>(it.head) * D + lane * 8;
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const uint64_t row = r0 + k * kGroups;
-      slot[k] = -1;
-      if (row < total) {
-        ref[k] = row_ref(p, static_cast<uint32_t>(row));
-        slot[k] = slot_of(p, ref[k].token);
-        if (active) {
-          const T* src = static_cast<const T*>(p.src[ref[k].half]) +
-                         static_cast<int64_t>(ref[k].token) * p.token_stride[ref[k].half] +
-                         static_cast<int64_t>(ref[k].head) * p.head_size + lane * 8;
-          x[k] = load8<T, kVec>(src);
-        }
-        if (slot[k] >= p.num_rows) {
-          if (lane == 0) raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
-          slot[k] = -1;
-        }
+      for (int k = 0; k < kHeads; ++k) {
+        if (k < it.count) x[k] = load8<T, kVec>(src + k * D);
       }
     }
+    int32_t* row = p.cache + (it.half ? p.half_words : 0) + it.slot * p.row_words;
+    int32_t* codes = row + static_cast<int64_t>(it.head) * (D / 8) + lane;
+    int32_t* params = row + static_cast<int64_t>(p.num_heads) * (D / 8) + it.head;
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
+    for (int k = 0; k < kHeads; ++k) {
+      float lo, hi;
+      row_range<T, kGroup>(x[k], active, lo, hi);
       float v[8];
-      float lo = INFINITY, hi = -INFINITY;
-      if (active && slot[k] >= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_float(x[k].v[i]);
+      if (__any_sync(0xffffffffu, !(lo >= -65504.0f && hi <= 65504.0f))) {
+        lo = INFINITY;
+        hi = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          v[i] = finite_half_range(to_float(x[k].v[i]));
-          lo = fminf(lo, v[i]);
-          hi = fmaxf(hi, v[i]);
+          v[i] = finite_half_range(v[i]);
+          if (active) {
+            lo = fminf(lo, v[i]);
+            hi = fmaxf(hi, v[i]);
+          }
+        }
+#pragma unroll
+        for (int o = kGroup / 2; o > 0; o >>= 1) {
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
       }
-#pragma unroll
-      for (int o = kGroup / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      if (!active || slot[k] < 0) continue;
-      const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
-      // + 0: a zero of either sign is kept as +0, so equal rows have equal words
-      const float z = __half2float(__float2half_rn(lo)) + 0.0f;
-      const __half zh = __float2half_rn(z);
-      const float s = __half2float(sh);
-      uint32_t word = 0;
-      if (s > 0.0f) {
-        const float inv = __frcp_rn(s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) word |= code_of(v[i], z, s, inv) << (4 * i);
-      }
-      int32_t* dst = p.cache + (ref[k].half ? p.half_words : 0) + slot[k] * p.row_words;
-      dst[static_cast<int64_t>(ref[k].head) * words + lane] = static_cast<int32_t>(word);
-      if (lane == 0) {
-        dst[static_cast<int64_t>(p.num_heads) * words + ref[k].head] = static_cast<int32_t>(
-            static_cast<uint32_t>(__half_as_ushort(sh)) |
-            (static_cast<uint32_t>(__half_as_ushort(zh)) << 16));
+      if (k < it.count && active) {
+        const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
+        // + 0: a zero of either sign is kept as +0, so equal rows have equal words
+        const float z = __half2float(__float2half_rn(lo)) + 0.0f;
+        const float s = __half2float(sh);
+        const uint32_t word = s > 0.0f ? word_of(v, z, s) : 0;
+        codes[k * (D / 8)] = static_cast<int32_t>(word);
+        if (lane == 0) {
+          params[k] = static_cast<int32_t>(
+              static_cast<uint32_t>(__half_as_ushort(sh)) |
+              (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(z))) << 16));
+        }
       }
     }
   }
 }
 
-template <typename T, int kGroup, bool kVec>
+template <typename T, int kGroup, int kHeads, bool kVec>
 __global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4Params p) {
   const int lane = threadIdx.x % kGroup;
-  if (lane * 8 >= p.head_size) return;
-  const uint32_t total = 2 * p.rows_per_half;
+  const int D = p.head_size;
+  if (lane * 8 >= D) return;
   constexpr uint32_t kGroups = kThreads / kGroup;
-  const int words = p.head_size / 8;
-  for (uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * (kGroups * kRows) + threadIdx.x / kGroup;
-       r0 < total; r0 += static_cast<uint64_t>(gridDim.x) * kGroups * kRows) {
-    uint32_t word[kRows], par[kRows];
-    int64_t slot[kRows];
-    RowRef ref[kRows];
+  for (uint64_t at = static_cast<uint64_t>(blockIdx.x) * kGroups + threadIdx.x / kGroup;
+       at < 2ull * p.items_per_half; at += static_cast<uint64_t>(gridDim.x) * kGroups) {
+    const Item it = item_of<kHeads>(p, at, lane == 0);
+    if (it.count == 0) continue;
+    const int32_t* row = p.cache + (it.half ? p.half_words : 0) + it.slot * p.row_words;
+    const int32_t* codes = row + static_cast<int64_t>(it.head) * (D / 8) + lane;
+    const int32_t* params = row + static_cast<int64_t>(p.num_heads) * (D / 8) + it.head;
+    uint32_t word[kHeads], par[kHeads];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const uint64_t row = r0 + k * kGroups;
-      slot[k] = -1;
-      if (row < total) {
-        ref[k] = row_ref(p, static_cast<uint32_t>(row));
-        slot[k] = slot_of(p, ref[k].token);
-        if (slot[k] >= p.num_rows) {
-          if (lane == 0) raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
-          slot[k] = -1;
-        }
+    for (int k = 0; k < kHeads; ++k) {
+      if (k < it.count) {
+        word[k] = static_cast<uint32_t>(codes[k * (D / 8)]);
+        par[k] = static_cast<uint32_t>(params[k]);
       }
     }
+    T* dst = static_cast<T*>(it.half ? p.dst[1] : p.dst[0]) +
+             static_cast<int64_t>(it.token) * (it.half ? p.token_stride[1] : p.token_stride[0]) +
+             static_cast<int64_t>(it.head) * D + lane * 8;
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (slot[k] >= 0) {
-        const int32_t* src = p.cache + (ref[k].half ? p.half_words : 0) + slot[k] * p.row_words;
-        word[k] = static_cast<uint32_t>(src[static_cast<int64_t>(ref[k].head) * words + lane]);
-        par[k] = static_cast<uint32_t>(
-            src[static_cast<int64_t>(p.num_heads) * words + ref[k].head]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (slot[k] < 0) continue;
+    for (int k = 0; k < kHeads; ++k) {
+      if (k >= it.count) continue;
       const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(par[k])));
       const float z = __half2float(__ushort_as_half(static_cast<unsigned short>(par[k] >> 16)));
       Eight<T> out;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        out.v[i] = from_float<T>(__fmaf_rn(static_cast<float>((word[k] >> (4 * i)) & 15u), s, z));
+        // 2^23 + code as a float's bits, less 2^23: the code, exactly
+        const float c = __uint_as_float(((word[k] >> (4 * i)) & 15u) | 0x4B000000u) - 8388608.0f;
+        out.v[i] = from_float<T>(__fmaf_rn(c, s, z));
       }
-      T* dst = static_cast<T*>(p.dst[ref[k].half]) +
-               static_cast<int64_t>(ref[k].token) * p.token_stride[ref[k].half] +
-               static_cast<int64_t>(ref[k].head) * p.head_size + lane * 8;
-      store8<T, kVec>(dst, out);
+      store8<T, kVec>(dst + k * D, out);
     }
+  }
+}
+
+template <typename T, int kGroup, int kHeads, bool kVec>
+void launch_items(Kv4Params p, bool store, cudaStream_t stream) {
+  const uint32_t per_token = static_cast<uint32_t>((p.num_heads + kHeads - 1) / kHeads);
+  p.items_per_half = static_cast<uint32_t>(p.num_tokens) * per_token;
+  p.div_items = FastDiv(per_token);
+  constexpr uint32_t kPerCta = kThreads / kGroup;
+  const uint64_t want = (2ull * p.items_per_half + kPerCta - 1) / kPerCta;
+  const uint64_t most = static_cast<uint64_t>(current_sm_count()) * 8;
+  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
+  if (store) {
+    kv4_store_kernel<T, kGroup, kHeads, kVec><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    kv4_load_kernel<T, kGroup, kHeads, kVec><<<grid, kThreads, 0, stream>>>(p);
   }
 }
 
 template <typename T, int kGroup, bool kVec>
 void launch(const Kv4Params& p, bool store, cudaStream_t stream) {
-  constexpr uint32_t kPerCta = kThreads / kGroup * kRows;
-  const uint64_t want = (2ull * p.rows_per_half + kPerCta - 1) / kPerCta;
-  const uint64_t most = static_cast<uint64_t>(current_sm_count()) * 8;
-  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
-  if (store) {
-    kv4_store_kernel<T, kGroup, kVec><<<grid, kThreads, 0, stream>>>(p);
+  // Few head rows are spread over the lanes; many are taken kMost at a time.
+  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.num_heads * 2;
+  const int64_t lanes = static_cast<int64_t>(current_sm_count()) * 1024;
+  if (p.num_heads == 1 || rows * kGroup <= lanes) {
+    launch_items<T, kGroup, 1, kVec>(p, store, stream);
   } else {
-    kv4_load_kernel<T, kGroup, kVec><<<grid, kThreads, 0, stream>>>(p);
+    launch_items<T, kGroup, kMost, kVec>(p, store, stream);
   }
 }
 
@@ -345,8 +420,6 @@ int run(const char* name, const void* key_in, const void* value_in, void* key_ou
   p.num_tokens = static_cast<int32_t>(num_tokens);
   p.num_heads = static_cast<int32_t>(num_heads);
   p.head_size = static_cast<int32_t>(head_size);
-  p.rows_per_half = static_cast<uint32_t>(num_tokens * num_heads);
-  p.div_heads = FastDiv(static_cast<uint32_t>(num_heads));
   p.status = device_status_ptr();
   if (p.status == nullptr) return LMCB_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
