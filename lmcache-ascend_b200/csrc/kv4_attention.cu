@@ -33,9 +33,9 @@
 // times the bytes read, for query tiles of 8 rows out of its 128.
 //
 // A CTA works on all KV heads of a token range (up to 8), so it reads whole
-// rows: a producer warp brings the rows of a page with one bulk copy for K and
-// one for V into a ring of stages, and eight warps take a head each (with
-// fewer heads, several warps take a head's tokens in turn). The tiles of all
+// rows: one warp at a time, in turn, brings the rows of a page with one bulk
+// copy for K and one for V into a ring of stages, and eight warps take a head
+// each (with fewer heads, several warps share a head's tokens). The tiles of all
 // requests are one line that is cut into equal pieces, so ragged lengths
 // leave no CTA idle; a second kernel joins requests that were cut.
 #include <climits>
@@ -49,8 +49,8 @@ namespace lmcb {
 namespace kv4 {
 namespace {
 
-constexpr int kWarps = 8;                    // consumers
-constexpr int kThreads = (kWarps + 1) * 32;  // and the producer
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMaxStages = 8;
 constexpr int kMaxRounds = 4;  // stage tokens / 32 at most
 
@@ -83,10 +83,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ void consumer_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
-}
-
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* src) {
   if constexpr (N % 4 == 0) {
@@ -108,13 +104,10 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* src)
 struct Line {
   const int32_t* prefix;  // [batch + 1] in shared memory
   int32_t batch, per_group;
-  int64_t at, end;
-  int first;
+  int64_t begin, end;
 
-  // The next piece of a unit; false at the end.
-  __device__ __forceinline__ bool next(int& group, int& b, int32_t& t0, int32_t& t1, int& slot,
-                                       int cta) {
-    if (at >= end) return false;
+  // The unit of the tile at `at`, and its tile in it.
+  __device__ __forceinline__ void find(int64_t at, int& group, int& b, int32_t& t) const {
     group = static_cast<int>(at / per_group);
     const int32_t in_group = static_cast<int32_t>(at - static_cast<int64_t>(group) * per_group);
     int lo = 0, hi = batch;  // prefix[lo] <= in_group < prefix[hi]
@@ -123,15 +116,7 @@ struct Line {
       if (prefix[mid] <= in_group) lo = mid; else hi = mid;
     }
     b = lo;
-    const int32_t tiles = prefix[lo + 1] - prefix[lo];
-    t0 = in_group - prefix[lo];
-    const int64_t left = end - at;
-    t1 = left < tiles - t0 ? t0 + static_cast<int32_t>(left) : tiles;
-    // a whole unit goes to the output; a piece is this CTA's first or its last
-    slot = t0 == 0 && t1 == tiles ? -1 : 2 * cta + (first ? 0 : 1);
-    first = 0;
-    at += t1 - t0;
-    return true;
+    t = in_group - prefix[lo];
   }
 };
 
@@ -496,7 +481,7 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
 #pragma unroll
       for (int c = 0; c < 2; ++c) s_m[(turn * heads + head) * R + n * 8 + 2 * t + c] = st.m[n][c];
   }
-  consumer_sync();
+  __syncthreads();
   const float unit = st.value_unit(), unit16 = unit * 0.0625f;
   float f[NT][2];
 #pragma unroll
@@ -535,9 +520,9 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
           }
         }
     }
-    consumer_sync();
+    __syncthreads();
   }
-  for (int i = threadIdx.x; i < heads * p.rows * (D / 4); i += kWarps * 32) {
+  for (int i = threadIdx.x; i < heads * p.rows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), e = (i % (D / 4)) * 4;
     const int h = row / p.rows, col = row % p.rows;
     const int kv_head = group * heads + h;
@@ -562,112 +547,124 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
       }
     }
   }
-  consumer_sync();  // the buffer is used again by the next unit
+  __syncthreads();  // the buffer is used again by the next unit
 }
 
-// The producer warp: the rows of every tile of the line, in order, into the
-// ring.
-__device__ __forceinline__ bool produce(const DecodeParams& p, Line line, uint8_t* ring,
-                                        uint64_t* full, uint64_t* empty,
-                                        uint32_t (*valid)[kMaxRounds], int half_size,
-                                        uint32_t& issued) {
+// Shared state of the ring. Tile j of this CTA goes into stage j % stages.
+struct Ring {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint32_t valid[kMaxStages][kMaxRounds];  // tokens that are there, a bit each
+  uint32_t issued;                         // tiles brought so far
+};
+
+// One warp brings tile `j`: it finds the rows of the tile's tokens, waits for
+// the stage and starts the copies.
+__device__ __forceinline__ bool produce(const DecodeParams& p, const Line& line, uint32_t j,
+                                        uint8_t* data, Ring& ring, int half_size) {
   const AttnParams& a = p.a;
   const int lane = threadIdx.x % 32;
   const int rounds = (p.stage_tokens + 31) / 32;
   const uint32_t row_bytes = static_cast<uint32_t>(a.row_words) * 4;
+  const uint32_t stage = j % p.stages, turn = j / p.stages;
+  int group, b;
+  int32_t t;
+  line.find(line.begin + j, group, b, t);
+  const Request rq = load_request(a, b, false);
+  const KeyRange range = request_range(a, rq);
+  const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_stride;
+  int32_t row[kMaxRounds];
+  uint32_t there[kMaxRounds];
+  uint32_t count = 0;
+#pragma unroll
+  for (int r = 0; r < kMaxRounds; ++r) {
+    row[r] = -1;
+    there[r] = 0;
+    if (r < rounds) {
+      const int tok = r * 32 + lane;
+      if (tok < p.stage_tokens) row[r] = row_of(a, table, range, t * p.stage_tokens + tok);
+      there[r] = __ballot_sync(0xffffffffu, row[r] >= 0);
+      count += __popc(there[r]);
+    }
+  }
+  // what is copied of a row: all of it, or this group's codes and the 16-byte
+  // pieces that hold its parameters
+  const int heads = min(p.heads, a.kv_heads - group * p.heads);
+  const uint32_t code_at = static_cast<uint32_t>(group * p.heads * half_size);
+  const uint32_t code_bytes = static_cast<uint32_t>(heads * half_size);
+  const uint32_t par = static_cast<uint32_t>(a.kv_heads * half_size + group * p.heads * 4);
+  const uint32_t par_at = par & ~15u;
+  const uint32_t par_bytes = ((par + heads * 4 + 15) & ~15u) - par_at;
+  const uint32_t tok_bytes = 2 * (p.groups == 1 ? row_bytes : code_bytes + par_bytes);
+  if (turn > 0 && !mbar_wait(&ring.empty[stage], (turn - 1) & 1)) return false;
+  uint64_t* full = &ring.full[stage];
+  if (lane == 0) {
+#pragma unroll
+    for (int r = 0; r < kMaxRounds; ++r) {
+      if (r < rounds) ring.valid[stage][r] = there[r];
+    }
+    atomicMax(&ring.issued, j + 1);
+    mbar_arrive_expect_tx(full, count * tok_bytes);
+  }
+  __syncwarp();
   const uint8_t* k_rows = reinterpret_cast<const uint8_t*>(a.cache);
   const uint8_t* v_rows = k_rows + a.half_words * 4;
-  int group, b, slot;
-  int32_t t0, t1;
-  uint32_t stage = 0, phase = 0;
-  issued = 0;
-  while (line.next(group, b, t0, t1, slot, blockIdx.x)) {
-    const Request rq = load_request(a, b, false);
-    const KeyRange range = request_range(a, rq);
-    const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_stride;
-    // what is copied of a row: all of it, or this group's codes and the 16-byte
-    // pieces that hold its parameters
-    const int heads = min(p.heads, a.kv_heads - group * p.heads);
-    const uint32_t code_at = static_cast<uint32_t>(group * p.heads * half_size);
-    const uint32_t code_bytes = static_cast<uint32_t>(heads * half_size);
-    const uint32_t par = static_cast<uint32_t>(a.kv_heads * half_size + group * p.heads * 4);
-    const uint32_t par_at = par & ~15u;
-    const uint32_t par_bytes = ((par + heads * 4 + 15) & ~15u) - par_at;
-    const uint32_t tok_bytes = 2 * (p.groups == 1 ? row_bytes : code_bytes + par_bytes);
-    for (int32_t t = t0; t < t1; ++t) {
-      int32_t row[kMaxRounds];
-      uint32_t there[kMaxRounds];
-      uint32_t count = 0;
+  uint8_t* dst = data + stage * p.stage_bytes;
+  const uint32_t v_off = static_cast<uint32_t>(p.stage_tokens * p.tok_stride);
 #pragma unroll
-      for (int r = 0; r < kMaxRounds; ++r) {
-        row[r] = -1;
-        if (r < rounds) {
-          const int tok = r * 32 + lane;
-          if (tok < p.stage_tokens) {
-            row[r] = row_of(a, table, range, t * p.stage_tokens + tok);
-          }
-          there[r] = __ballot_sync(0xffffffffu, row[r] >= 0);
-          count += __popc(there[r]);
-        }
+  for (int r = 0; r < kMaxRounds; ++r) {
+    if (r >= rounds) continue;
+    uint8_t* to = dst + (r * 32 + lane) * p.tok_stride;
+    const int64_t from = static_cast<int64_t>(row[r]) * row_bytes;
+    if (p.groups == 1) {
+      // runs of rows that follow one another in the cache: one copy each
+      const int32_t prev = __shfl_up_sync(0xffffffffu, row[r], 1);
+      const bool start = row[r] >= 0 && (lane == 0 || row[r] != prev + 1);
+      const uint32_t stops = __ballot_sync(0xffffffffu, start) | ~there[r];
+      if (start) {
+        const uint32_t above = lane == 31 ? 0 : stops >> (lane + 1);
+        const uint32_t n = above ? __ffs(above) : 32 - lane;
+        bulk_load(to, k_rows + from, n * row_bytes, full);
+        bulk_load(to + v_off, v_rows + from, n * row_bytes, full);
       }
-      if (!mbar_wait(&empty[stage], phase ^ 1)) return false;
-      if (lane == 0) {
-#pragma unroll
-        for (int r = 0; r < kMaxRounds; ++r) {
-          if (r < rounds) valid[stage][r] = there[r];
-        }
-        mbar_arrive_expect_tx(&full[stage], count * tok_bytes);
-      }
-      __syncwarp();
-      uint8_t* dst = ring + stage * p.stage_bytes;
-      const uint32_t v_off = static_cast<uint32_t>(p.stage_tokens * p.tok_stride);
-#pragma unroll
-      for (int r = 0; r < kMaxRounds; ++r) {
-        if (r >= rounds) continue;
-        const int tok = r * 32 + lane;
-        uint8_t* to = dst + tok * p.tok_stride;
-        const int64_t from = static_cast<int64_t>(row[r]) * row_bytes;
-        if (p.groups == 1) {
-          // runs of rows that follow one another in the cache: one copy each
-          const int32_t prev = __shfl_up_sync(0xffffffffu, row[r], 1);
-          const bool start = row[r] >= 0 && (lane == 0 || row[r] != prev + 1);
-          const uint32_t stops = __ballot_sync(0xffffffffu, start) | ~there[r];
-          if (start) {
-            const uint32_t above = lane == 31 ? 0 : stops >> (lane + 1);
-            const uint32_t n = above ? __ffs(above) : 32 - lane;
-            bulk_load(to, k_rows + from, n * row_bytes, &full[stage]);
-            bulk_load(to + v_off, v_rows + from, n * row_bytes, &full[stage]);
-          }
-        } else if (row[r] >= 0) {
-          bulk_load(to, k_rows + from + code_at, code_bytes, &full[stage]);
-          bulk_load(to + p.heads * half_size, k_rows + from + par_at, par_bytes, &full[stage]);
-          bulk_load(to + v_off, v_rows + from + code_at, code_bytes, &full[stage]);
-          bulk_load(to + v_off + p.heads * half_size, v_rows + from + par_at, par_bytes,
-                    &full[stage]);
-        }
-      }
-      ++issued;
-      if (++stage == static_cast<uint32_t>(p.stages)) stage = 0, phase ^= 1;
+    } else if (row[r] >= 0) {
+      bulk_load(to, k_rows + from + code_at, code_bytes, full);
+      bulk_load(to + p.heads * half_size, k_rows + from + par_at, par_bytes, full);
+      bulk_load(to + v_off, v_rows + from + code_at, code_bytes, full);
+      bulk_load(to + v_off + p.heads * half_size, v_rows + from + par_at, par_bytes, full);
     }
   }
   return true;
 }
 
+// The tiles of this CTA. In step j every warp works on tile j, and one of them,
+// in turn, first brings the tile that takes the place of tile j - 1: the warps
+// may drift a tile apart, and no warp stays behind for being the producer.
 template <typename T, int D, int NT, int ST>
-__device__ __forceinline__ bool consume(const DecodeParams& p, Line line, const uint8_t* ring,
-                                        uint64_t* full, uint64_t* empty,
-                                        const uint32_t (*valid)[kMaxRounds], float* merge) {
+__device__ __forceinline__ bool run_line(const DecodeParams& p, const Line& line, uint8_t* data,
+                                         Ring& ring, float* merge) {
   const AttnParams& a = p.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int head = warp % p.heads, turn = warp / p.heads;
   const int first = turn * ST * 16;  // this warp's tokens of a stage
+  const uint32_t count = static_cast<uint32_t>(line.end - line.begin);
   bool ok = true;
-  int group, b, slot;
-  int32_t t0, t1;
+  if (warp < p.stages && static_cast<uint32_t>(warp) < count) {
+    produce(p, line, warp, data, ring, D / 2);
+  }
+  __syncthreads();
   uint32_t stage = 0, phase = 0;
   Query<D, NT> q;
   Running<D, NT> st;
-  while (line.next(group, b, t0, t1, slot, blockIdx.x)) {
+  for (uint32_t j = 0; j < count;) {
+    int group, b;
+    int32_t t;
+    line.find(line.begin + j, group, b, t);
+    const int32_t tiles = line.prefix[b + 1] - line.prefix[b];
+    const uint32_t steps = min(static_cast<uint32_t>(tiles - t), count - j);
+    // a whole unit goes to the output; a piece is this CTA's first or its last
+    const int slot = steps == static_cast<uint32_t>(tiles)
+                         ? -1
+                         : 2 * static_cast<int>(blockIdx.x) + (j == 0 ? 0 : 1);
     const Request rq = load_request(a, b, false);
     const KeyRange range = request_range(a, rq);
     const int kv_head = group * p.heads + head;
@@ -680,27 +677,29 @@ __device__ __forceinline__ bool consume(const DecodeParams& p, Line line, const 
                                   ((a.kv_heads * (D / 2) + group * p.heads * 4) & 15) + head * 4;
     if (working) load_unit_query<T, D, NT>(a, rq, kv_head, q);
     st.reset();
-    for (int32_t t = t0; t < t1 && ok; ++t) {
-      ok = mbar_wait(&full[stage], phase);
-      if (!ok) break;
-      if (working) {
-        const uint8_t* at = ring + stage * p.stage_bytes;
+    for (const uint32_t j_end = j + steps; j < j_end; ++j, ++t) {
+      if (j > 0 && j % kWarps == static_cast<uint32_t>(warp) && j - 1 + p.stages < count && ok) {
+        ok = produce(p, line, j - 1 + p.stages, data, ring, D / 2);
+      }
+      ok = ok && mbar_wait(&ring.full[stage], phase);
+      if (working && ok) {
+        const uint8_t* at = data + stage * p.stage_bytes;
         bool all = !mask;
 #pragma unroll
         for (int u = 0; u < ST; ++u) {
           const int tok = first + u * 16;
-          all = all && ((valid[stage][tok / 32] >> (tok % 32)) & 0xffffu) == 0xffffu;
+          all = all && ((ring.valid[stage][tok / 32] >> (tok % 32)) & 0xffffu) == 0xffffu;
         }
         if (all) {
-          take_tile<D, NT, ST, true>(p, at, valid[stage], first, code_off, par_off, range,
+          take_tile<D, NT, ST, true>(p, at, ring.valid[stage], first, code_off, par_off, range,
                                      t * p.stage_tokens, false, q, st);
         } else {
-          take_tile<D, NT, ST, false>(p, at, valid[stage], first, code_off, par_off, range,
+          take_tile<D, NT, ST, false>(p, at, ring.valid[stage], first, code_off, par_off, range,
                                       t * p.stage_tokens, mask, q, st);
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (lane == 0) mbar_arrive(&ring.empty[stage]);
       if (++stage == static_cast<uint32_t>(p.stages)) stage = 0, phase ^= 1;
     }
     // the warp's own sums over its tokens
@@ -733,11 +732,9 @@ template <typename T, int D, int NT, int ST>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NT>())
 kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(16) uint8_t decode_smem[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
-  __shared__ uint32_t valid[kMaxStages][kMaxRounds];
-  __shared__ int32_t s_warp[kWarps + 1];
-  uint8_t* ring = decode_smem;
-  float* merge = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes);
+  __shared__ Ring ring;
+  __shared__ int32_t s_warp[kWarps];
+  float* merge = reinterpret_cast<float*>(decode_smem + p.stages * p.stage_bytes);
   int32_t* prefix = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(merge) +
                                                merge_bytes<D, NT>(p.heads));
   const AttnParams& a = p.a;
@@ -745,9 +742,10 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   pdl_launch_dependents();  // the joining kernel may take its place; it waits for this one
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kWarps);
+      mbar_init(&ring.full[s], 1);
+      mbar_init(&ring.empty[s], kWarps);
     }
+    ring.issued = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   int32_t base = 0;
@@ -764,7 +762,7 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
     if (lane == 31) s_warp[warp] = sum;
     __syncthreads();
     int32_t before = base;
-    for (int w = 0; w <= kWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += s_warp[w];
       base += s_warp[w];
     }
@@ -783,23 +781,20 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   line.prefix = prefix;
   line.batch = a.batch;
   line.per_group = base;
-  line.at = total * blockIdx.x / n;
+  line.begin = total * blockIdx.x / n;
   line.end = total * (blockIdx.x + 1) / n;
-  line.first = 1;
-  if (warp == kWarps) {
-    uint32_t issued = 0;
-    if (!produce(p, line, ring, full, empty, valid, D / 2, issued)) {
-      if (lane == 0) raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
+  const bool ok = run_line<T, D, NT, ST>(p, line, decode_smem, ring, merge);
+  if (__syncthreads_or(!ok)) {
+    if (threadIdx.x == 0) {
+      raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
       // copies in flight write to this CTA's shared memory: they land first
-      for (int s = 0; s < p.stages; ++s) {
-        if (issued > static_cast<uint32_t>(s)) {
-          const uint32_t turn = (issued - 1 - s) / p.stages;
-          mbar_wait(&full[s], turn & 1);
-        }
+      const uint32_t issued = ring.issued;
+      for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0;
+           j < issued; ++j) {
+        mbar_wait(&ring.full[j % p.stages], (j / p.stages) & 1);
       }
     }
-  } else if (!consume<T, D, NT, ST>(p, line, ring, full, empty, valid, merge)) {
-    if (lane == 0) raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
+    __syncthreads();
   }
 }
 
