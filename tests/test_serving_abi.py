@@ -130,7 +130,7 @@ def attn_args(**kw):
     (dict(ts=15), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(blocks=1 << 28), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(cols=1 << 28, ts=1 << 28), abi.LMCB_ERR_INVALID_ARGUMENT),
-    (dict(batch=65536, rows=65536), abi.LMCB_ERR_INVALID_ARGUMENT),
+    (dict(batch=4097, rows=4097), abi.LMCB_ERR_CAPACITY),
     (dict(q=None), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(lens=None), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(cache=P + 4), abi.LMCB_ERR_INVALID_ARGUMENT),
@@ -144,11 +144,15 @@ def test_kv4_attention_refuses(kw, status):
 
 def test_workspace_size():
     n = ctypes.c_size_t(7)
-    # one step of tiles a request: nothing is split
-    abi.call("lmcb_kv4_attention_workspace", 4, 1, 16, 8, 32, 128, 0, 0, ctypes.byref(n))
-    assert n.value == 0
-    abi.call("lmcb_kv4_attention_workspace", 4, 1, 1 << 20, 8, 32, 128, 0, 0, ctypes.byref(n))
-    assert 0 < n.value < 64 << 20
+    for batch, query, length in ((4, 1, 16), (4, 1, 1 << 20), (1, 8, 1 << 20), (1, 1, 0)):
+        abi.call("lmcb_kv4_attention_workspace", batch, query, length, 8, 32, 128, 0, 0,
+                 ctypes.byref(n))
+        assert 0 < n.value < 64 << 20
+    # no request, and units enough for every CTA: nothing is split
+    for batch, query in ((0, 1), (64, 4096)):
+        abi.call("lmcb_kv4_attention_workspace", batch, query, 1 << 20, 8, 32, 128, 0, 0,
+                 ctypes.byref(n))
+        assert n.value == 0
     refused("lmcb_kv4_attention_workspace", abi.LMCB_ERR_INVALID_ARGUMENT, 4, 1, 16, 8, 32, 100, 0,
             0, ctypes.byref(n))
     refused("lmcb_kv4_attention_workspace", abi.LMCB_ERR_INVALID_ARGUMENT, 4, 1, 16, 8, 32, 128, 0,
