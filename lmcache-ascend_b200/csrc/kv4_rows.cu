@@ -16,16 +16,21 @@
 // of their own size: dequantising V costs 128 rows nothing, where taking sv
 // into P, as the decode kernel does, would cost every element of S.
 //
-// Per tile and SM the tensor core needs 512 cycles, the exponentials 512 (16 a
-// cycle), and the rest of softmax and dequantisation about as many issue
-// slots. So two CTAs share an SM, each with its half of the tensor memory (two
-// S of 64 columns and O), and one computes softmax while the other's products
-// run: four warps of a CTA have a query row a thread, four bring the codes from
-// the pages and expand them to 16 bits into two stages of shared memory (128-
-// byte swizzled; a lane's 16-byte pieces of 4 tokens x 2 halves of a panel hit
-// all banks). S of the next tile is under way before softmax starts. O stays
-// in tensor memory; it is rescaled only when a row's reference grows by more
-// than 2^12, which P's range leaves room for.
+// A CTA has two such units (one for D = 256), 256 query rows, which share the
+// tiles. Per tile the tensor core needs 1024 cycles for them, the exponentials
+// 1024 (16 a cycle), the rest of softmax and the expanding of codes about as
+// many issue slots, and shared memory as many accesses of 128 bytes; so the
+// work is laid out to keep all four going at once:
+//  - Q, as P, is read from tensor memory, and shared memory holds only K and
+//    V, up to six stages of them: four warps bring the codes from the pages and
+//    expand them (128-byte swizzle; a lane's 16-byte pieces of 4 tokens x 2
+//    halves of a panel hit all banks), far ahead of the products;
+//  - one warp issues products: while one unit computes softmax, the other's
+//    P V and next Q K^T run (P takes the place of S);
+//  - four warps a unit compute softmax. A lane has 4 rows x 16 tokens, not one
+//    row x 64 tokens, and so loads a quarter of the tokens' scales.
+// O stays in tensor memory; it is rescaled only when a row's reference grows by
+// more than 2^8, which P's range leaves room for.
 #include <climits>
 
 #include "kv4_attention.cuh"
@@ -35,16 +40,18 @@ namespace lmcb {
 namespace kv4 {
 namespace {
 
-constexpr int kRows = 128;   // query rows of a unit
-constexpr int kTok = 64;     // cache tokens of a tile
-constexpr int kThreads = 256;
-constexpr float kSlack = 12.0f;  // log2 of how far P may exceed 1
+constexpr int kRows = 128;  // query rows of a unit
+constexpr int kTok = 64;    // cache tokens of a tile
+// How far P may exceed 1 before O is rescaled, log2: by a row's maximum, and
+// by the exponent of V.
+constexpr float kSlack = 8.0f;
+constexpr int kExpSlack = 4;
 
 struct RowsParams {
   AttnParams a;
   int32_t splits;  // CTAs that share a unit's tiles
-  float* part;     // [unit][splits][kRows][D + 4]
-  int32_t row_tiles;
+  float* part;        // [CTA's rows][splits][rows][D + 4]
+  int32_t row_tiles;  // CTAs a request's rows may take
 };
 
 // Packed pairs of fp32.
@@ -102,6 +109,32 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[
       : "memory");
 }
 
+// 16 lanes x 64 columns: lane (g, t) of the warp has, of each 8 columns, columns
+// 2 t and 2 t + 1 of lanes g (r[4 n], r[4 n + 1]) and g + 8 (r[4 n + 2, 3]).
+__device__ __forceinline__ void tmem_load_rows(uint32_t (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+
+// 16 lanes x 32 columns: lane (g, t) has, of each 4 columns, column t of lanes g
+// (r[2 n]) and g + 8 (r[2 n + 1]).
+__device__ __forceinline__ void tmem_store_rows(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_load() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -132,14 +165,6 @@ __host__ __device__ constexpr uint32_t instruction(int n, bool across) {
          (static_cast<uint32_t>(kRows / 16) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr,
-                                       bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(instr), "r"(add ? 1u : 0u)
-      : "memory");
-}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr,
                                        bool add) {
   asm volatile(
@@ -160,24 +185,30 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 
 template <int D>
 struct Layout {
-  static constexpr int kPanels = D / 64;                     // of 64 values, 128 bytes a row
-  static constexpr int kQPanel = kRows * 128;
+  static constexpr int kUnits = D <= 128 ? 2 : 1;  // of a CTA
+  static constexpr int kPanels = D / 64;           // of 64 values, 128 bytes a token
   static constexpr int kPanel = kTok * 128;
-  static constexpr int kStage = kPanels * kPanel;
-  static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kPanels * kQPanel;
-  static constexpr int kV = kK + 2 * kStage;
-  static constexpr int kBytes = kV + 2 * kStage;
-  static constexpr uint32_t kColumns = D <= 128 ? 256 : 512;  // tensor memory
-  static constexpr uint32_t kO = 2 * kTok;                    // its columns behind two S
+  static constexpr int kV = kPanels * kPanel;      // V behind K in a stage
+  static constexpr int kStage = 2 * kV;
+  static constexpr int kStages = D <= 128 ? 6 : 3;
+  static constexpr int kWarps = kUnits * 4 + 4 + 1;  // softmax, bringing, products
+  static constexpr int kThreads = kWarps * 32;
+  // Tensor memory of a unit: S (and P in its first half), Q, O.
+  static constexpr uint32_t kUnit = 256;
+  static constexpr uint32_t kQ = kTok;
+  static constexpr uint32_t kO = D <= 128 ? 128 : 192;
+  static constexpr uint32_t kColumns = 512;
 };
 
+constexpr int kMaxStages = 6;
+
 struct Control {
-  uint64_t kfull[2], vfull[2], qkdone[2], pvdone[2], drained;
-  float4 kpar[2][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
-  uint32_t valid[2][4];      // a bit a token, 16 tokens each
-  int32_t vexp[2][4];        // e of 16 tokens
-  float2 row[kRows];         // a, sum of q 2^-24
+  uint64_t full[kMaxStages], free[kMaxStages], sready[2], pready[2], drained;
+  float4 kpar[kMaxStages][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
+  uint32_t valid[kMaxStages][4];      // two bits a token, 16 tokens each
+  int32_t vexp[kMaxStages][4];        // e of 16 tokens
+  float2 row[2 * kRows];              // a, sum of q 2^-24; at the end m, l
+  float alpha[2 * kRows];
   uint32_t tmem;
 };
 
@@ -186,58 +217,56 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t piece) {
   return r * 128 + ((piece ^ (r & 7)) << 4);
 }
 
-// The unit's query rows, scaled to fp16, into shared memory: two threads a row.
+// A thread's query row, scaled to fp16, into tensor memory.
 template <typename T, int D>
-__device__ __forceinline__ void load_rows(const AttnParams& p, const Request& rq, int first_row,
-                                          int kv_head, uint8_t* smem, Control& ctl) {
-  const int r = threadIdx.x / 2, side = threadIdx.x % 2;
-  constexpr int N = D / 2;
-  const int flat = first_row + r;
+__device__ __forceinline__ void load_row(const AttnParams& p, const Request& rq, int flat,
+                                         int kv_head, uint32_t q_cols, float2& factors) {
   const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(flat)));
   const int head = kv_head * p.group + (flat - tok * p.group);
   const bool there = tok < rq.n;
   const T* src = static_cast<const T*>(p.q) + (rq.row0 + static_cast<int64_t>(tok)) * p.q_stride +
-                 static_cast<int64_t>(head) * D + side * N;
+                 static_cast<int64_t>(head) * D;
   float big = 0.0f;
   if (there) {
-#pragma unroll
-    for (int i = 0; i < N / 8; ++i) {
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
       float x[8];
       load_query<T, 8>(src + 8 * i, p.q_vec != 0, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[j]));
     }
   }
-  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
   const int e = min(max(((__float_as_int(big) >> 23) & 255) - 127, -100), 100);
   // the sign of the scale goes into the rows, so that the largest t is the
   // largest logit
   const float up = p.scale_log2 < 0.0f ? -pow2i(13 - e) : pow2i(13 - e);
   float sum = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < D / 2; c += 32) {
+    uint32_t q[32];
 #pragma unroll
-  for (int i = 0; i < N / 8; ++i) {
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (there) {
+    for (int i = 0; i < 8; ++i) {
       float x[8];
-      load_query<T, 8>(src + 8 * i, p.q_vec != 0, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+      if (there) load_query<T, 8>(src + 2 * c + 8 * i, p.q_vec != 0, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = __half2float(__float2half_rn(x[j] * up));
         sum += x[j];
       }
-      out = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1] * 0.0625f, x[5] * 0.0625f),
-                       pack_half2(x[2], x[6]), pack_half2(x[3] * 0.0625f, x[7] * 0.0625f));
+      q[4 * i] = pack_half2(x[0], x[4]);
+      q[4 * i + 1] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
+      q[4 * i + 2] = pack_half2(x[2], x[6]);
+      q[4 * i + 3] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
     }
-    const int at = side * (N / 8) + i;  // 8 values of the row
-    *reinterpret_cast<uint4*>(smem + Layout<D>::kQ + (at / 8) * Layout<D>::kQPanel +
-                              swizzled(r, at % 8)) = out;
+    __syncwarp();
+    tmem_store32(q_cols + c, q);
   }
-  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-  if (side == 0) {
-    // never zero, so that a key that is not seen stays at -inf
-    const float a = fmaxf(fabsf(p.scale_log2) * pow2i(e - 13) * 16777216.0f, 1.2e-38f);
-    ctl.row[r] = make_float2(a, sum * 5.9604645e-8f);
-  }
+  tmem_wait_store();
+  // a is never zero, so that a key that is not seen stays at -inf
+  factors = make_float2(fmaxf(fabsf(p.scale_log2) * pow2i(e - 13) * 16777216.0f, 1.2e-38f),
+                        sum * 5.9604645e-8f);
 }
 
 // ---------------------------------------------------------------------------
@@ -305,41 +334,42 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
                                       int kv_head, int32_t t0, int32_t tiles, uint8_t* smem,
                                       Control& ctl) {
   using L = Layout<D>;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32 - 4;
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32 - 4 * L::kUnits;
   const int tok = w * 16 + lane / 2;
   const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_stride;
   const int32_t* k_head = p.cache + static_cast<int64_t>(kv_head) * (D / 8);
   const int32_t* par = p.cache + static_cast<int64_t>(p.kv_heads) * (D / 8) + kv_head;
-  const auto row = [&](int32_t i) {
-    return i < tiles ? row_of(p, table, range, (t0 + i) * kTok + tok) : -1;
+  const int32_t size = static_cast<int32_t>(p.div_block.d);
+  // The page of this lane's token of tile i, unchecked: nothing waits for it
+  // before the tile's turn.
+  const auto page_of = [&](int32_t i) {
+    const int32_t v = (t0 + i) * kTok + tok;
+    if (i >= tiles || v >= range.count) return -1;
+    return __ldg(table + p.div_block.div(static_cast<uint32_t>(key_of(range, v))));
   };
-  // codes of the next tile and the row of the one after it are on their way
+  const auto row_in = [&](int32_t i, int32_t page) {
+    const int32_t v = (t0 + i) * kTok + tok;
+    if (i >= tiles || v >= range.count) return -1;
+    if (page < 0 || page >= p.num_blocks) {
+      raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
+      return -1;
+    }
+    const int32_t key = key_of(range, v);
+    return page * size +
+           (key - static_cast<int32_t>(p.div_block.div(static_cast<uint32_t>(key))) * size);
+  };
+  // codes of the next tile and the page of the one after it are on their way
   // while a tile is expanded
   Codes<D> next;
-  int32_t after = row(0);
-  fetch<D>(p, k_head, par, after, lane, next);
-  after = row(1);
+  int32_t page = page_of(0);
+  fetch<D>(p, k_head, par, row_in(0, page), lane, next);
+  page = page_of(1);
+  int stage = 0;
+  uint32_t phase = 1;  // parity of the stage's last use
   for (int32_t i = 0; i < tiles; ++i) {
-    const int buf = i & 1;
-    const uint32_t last = ((i >> 1) - 1) & 1;  // parity of the stage's last use
     const Codes<D> c = next;
-    fetch<D>(p, k_head, par, after, lane, next);
-    after = row(i + 2);
-    if (i >= 2 && !mbar_wait(&ctl.qkdone[buf], last)) return false;
-    uint8_t* k = smem + L::kK + buf * L::kStage;
-    const uint32_t piece = (lane % 2) * 4;
-#pragma unroll
-    for (int n = 0; n < L::kPanels; ++n) {
-      const uint32_t words[4] = {c.k[n].x, c.k[n].y, c.k[n].z, c.k[n].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<uint4*>(k + n * L::kPanel + swizzled(tok, piece + j)) =
-            expand_k(words[j]);
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.kfull[buf]);
+    fetch<D>(p, k_head, par, row_in(i + 1, page), lane, next);
+    page = page_of(i + 2);
     // the exponent above the largest value of these 16 tokens
     const float s = half_lo(c.vpar), z = half_hi(c.vpar);
     const float most = fmaxf(fabsf(z), fabsf(fmaf(15.0f, s, z)));
@@ -349,29 +379,102 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     const __half2 s2 = __half2half2(__float2half_rn(s * down));
     const __half2 z2 = __half2half2(__float2half_rn(z * down));
     const uint32_t there = __ballot_sync(0xffffffffu, c.there);
-    if (i >= 2 && !mbar_wait(&ctl.pvdone[buf], last)) return false;
-    uint8_t* v = smem + L::kV + buf * L::kStage;
+    if (i >= L::kStages && !mbar_wait(&ctl.free[stage], phase)) return false;
+    uint8_t* k = smem + stage * L::kStage;
+    const uint32_t piece = (lane % 2) * 4;
 #pragma unroll
     for (int n = 0; n < L::kPanels; ++n) {
-      const uint32_t words[4] = {c.v[n].x, c.v[n].y, c.v[n].z, c.v[n].w};
+      const uint32_t kw[4] = {c.k[n].x, c.k[n].y, c.k[n].z, c.k[n].w};
+      const uint32_t vw[4] = {c.v[n].x, c.v[n].y, c.v[n].z, c.v[n].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<uint4*>(v + n * L::kPanel + swizzled(tok, piece + j)) =
-            expand_v(words[j], s2, z2);
+        uint8_t* to = k + n * L::kPanel + swizzled(tok, piece + j);
+        *reinterpret_cast<uint4*>(to) = expand_k(kw[j]);
+        *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], s2, z2);
       }
     }
     if (lane % 2 == 0) {
-      float* to = reinterpret_cast<float*>(&ctl.kpar[buf][tok / 2]) + tok % 2;
+      float* to = reinterpret_cast<float*>(&ctl.kpar[stage][tok / 2]) + tok % 2;
       to[0] = half_lo(c.kpar);
       to[2] = half_hi(c.kpar);
     }
     if (lane == 0) {
-      ctl.valid[buf][w] = there;  // two bits a token
-      ctl.vexp[buf][w] = e;
+      ctl.valid[stage][w] = there;
+      ctl.vexp[stage][w] = e;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.vfull[buf]);
+    if (lane == 0) mbar_arrive(&ctl.full[stage]);
+    if (++stage == L::kStages) stage = 0, phase ^= 1;
+  }
+  return true;
+}
+
+// ---------------------------------------------------------------------------
+// The warp that issues the products
+// ---------------------------------------------------------------------------
+
+template <int D>
+__device__ __forceinline__ void issue_qk(uint32_t unit, uint32_t stage) {
+  using L = Layout<D>;
+  const uint64_t k = operand(stage, 0, 1024);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    mma_ts(unit, unit + L::kQ + i * 8, k + (((i / 4) * L::kPanel + (i % 4) * 32) >> 4),
+           instruction(kTok, false), i > 0);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void issue_pv(uint32_t unit, uint32_t stage, bool add) {
+  using L = Layout<D>;
+  const uint64_t v = operand(stage + L::kV, L::kPanel, 1024);
+#pragma unroll
+  for (int i = 0; i < kTok / 16; ++i) {
+    mma_ts(unit + L::kO, unit + i * 8, v + ((i * 16 * 128) >> 4), instruction(D, true),
+           add || i > 0);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, Control& ctl) {
+  using L = Layout<D>;
+  if (tiles == 0) return true;
+  const bool leader = threadIdx.x % 32 == 0;
+  const uint32_t tmem = ctl.tmem;
+  if (!mbar_wait(&ctl.full[0], 0)) return false;
+  fence_after();
+  if (leader) {
+    for (int u = 0; u < units; ++u) {
+      issue_qk<D>(tmem + u * L::kUnit, smem);
+      commit(&ctl.sready[u]);
+    }
+  }
+  __syncwarp();
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int32_t i = 0; i < tiles; ++i) {
+    const int next = stage + 1 == L::kStages ? 0 : stage + 1;
+    const uint32_t next_phase = stage + 1 == L::kStages ? phase ^ 1 : phase;
+    for (int u = 0; u < units; ++u) {
+      const uint32_t unit = tmem + u * L::kUnit;
+      if (!mbar_wait(&ctl.pready[u], i & 1)) return false;
+      fence_after();
+      if (leader) {
+        issue_pv<D>(unit, smem + stage * L::kStage, i > 0);
+        if (u == units - 1) commit(&ctl.free[stage]);
+      }
+      __syncwarp();
+      if (i + 1 < tiles) {
+        if (u == 0 && !mbar_wait(&ctl.full[next], next_phase)) return false;
+        // into the S whose P the product before reads: products run in order
+        if (leader) issue_qk<D>(unit, smem + next * L::kStage);
+      }
+      if (leader) commit(&ctl.sready[u]);
+      __syncwarp();
+    }
+    stage = next;
+    phase = next_phase;
   }
   return true;
 }
@@ -380,207 +483,193 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
 // The warps that have the query rows
 // ---------------------------------------------------------------------------
 
-template <int D>
-__device__ __forceinline__ void issue_qk(uint32_t tmem, uint32_t smem, int buf) {
-  using L = Layout<D>;
-  const uint64_t q = operand(smem + L::kQ, 0, 1024);
-  const uint64_t k = operand(smem + L::kK + buf * L::kStage, 0, 1024);
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const uint32_t in_panel = (i % 4) * 32;
-    mma_ss(tmem + buf * kTok, q + (((i / 4) * L::kQPanel + in_panel) >> 4),
-           k + (((i / 4) * L::kPanel + in_panel) >> 4), instruction(kTok, false), i > 0);
-  }
-}
-
-template <int D>
-__device__ __forceinline__ void issue_pv(uint32_t tmem, uint32_t smem, int buf, bool add) {
-  using L = Layout<D>;
-  const uint64_t v = operand(smem + L::kV + buf * L::kStage, L::kPanel, 1024);
-#pragma unroll
-  for (int i = 0; i < kTok / 16; ++i) {
-    mma_ts(tmem + L::kO, tmem + buf * kTok + i * 8, v + ((i * 16 * 128) >> 4),
-           instruction(D, true), add || i > 0);
-  }
-}
-
-// A thread's row: its reference m (log2) and E, the sum l in units of 2^m; O in
-// units of 2^(m + E).
-struct Row {
-  float a, qsum;
-  float m, l;
-  int e;
-  int32_t pos;
-};
-
+// Lane (g, t) has rows g + 8 k of the warp's 32, k < 4, and of each the tokens
+// 8 n + 2 t and 8 n + 2 t + 1 of a tile. A row's reference m (log2) and its sum
+// l, in units of 2^m; O is in units of 2^(m + e), e the same for all rows of a
+// warp.
 template <int D>
 __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& range, int32_t t0,
                                        int32_t tiles, int32_t pos_first, int32_t pos_last,
-                                       uint32_t smem, Control& ctl, Row& row) {
+                                       const Request& rq, int first_row, int unit, Control& ctl,
+                                       int& e_out) {
   using L = Layout<D>;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const uint32_t tmem = ctl.tmem;
-  const uint32_t mine = tmem + (static_cast<uint32_t>(w) << 21);  // lanes 32 w ...
-  bool ok = true;
-  if (w == 0 && tiles > 0) {
-    ok = mbar_wait(&ctl.kfull[0], 0);
-    if (ok && lane == 0) {
-      fence_after();
-      issue_qk<D>(tmem, smem, 0);
-      commit(&ctl.qkdone[0]);
-    }
-    __syncwarp();
+  const int lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
+  const int warp_row = unit * kRows + (threadIdx.x / 32 % 4) * 32;  // of the CTA's rows
+  const uint32_t mine = ctl.tmem + unit * L::kUnit +
+                        (static_cast<uint32_t>(threadIdx.x / 32 % 4) << 21);
+  float a[4], m[4], l[4];
+  float qsum[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = ctl.row[warp_row + g + 8 * k];
+    a[k] = f.x;
+    qsum[k] = f.y;
+    m[k] = -1e30f;
+    l[k] = 0.0f;
   }
+  int e = -100;
+  bool ok = true;
+  int stage = 0;
+  uint32_t phase = 0;
   for (int32_t i = 0; i < tiles; ++i) {
-    const int buf = i & 1;
-    const uint32_t parity = (i >> 1) & 1;
-    if (w == 0 && i + 1 < tiles && ok) {
-      ok = mbar_wait(&ctl.kfull[buf ^ 1], ((i + 1) >> 1) & 1);
-      if (ok && lane == 0) {
-        fence_after();
-        // into the S whose P the product before has read: products run in order
-        issue_qk<D>(tmem, smem, buf ^ 1);
-        commit(&ctl.qkdone[buf ^ 1]);
-      }
-      __syncwarp();
+    if (!mbar_wait(&ctl.full[stage], phase) || !mbar_wait(&ctl.sready[unit], i & 1)) {
+      ok = false;
+      break;
     }
-    ok = ok && mbar_wait(&ctl.vfull[buf], parity) && mbar_wait(&ctl.qkdone[buf], parity);
-    if (ok) {
-      fence_after();
-      uint32_t s[2][32];
-      tmem_load32(s[0], mine + buf * kTok);
-      tmem_load32(s[1], mine + buf * kTok + 32);
-      // is every key of the tile there and seen by every row?
-      const int32_t v0 = (t0 + i) * kTok;
-      const uint32_t there = ctl.valid[buf][0] & ctl.valid[buf][1] & ctl.valid[buf][2] &
-                             ctl.valid[buf][3];
-      const int32_t key0 = key_of(range, v0), key1 = key_of(range, v0 + kTok - 1);
-      const bool all = there == 0xffffffffu && key1 <= pos_first &&
-                       (p.window == 0 || key0 > pos_last - p.window || key1 < p.sinks);
-      tmem_wait_load();
-      uint64_t t[kTok / 2];
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      const uint64_t qsum = pair(row.qsum, row.qsum);
+    fence_after();
+    uint32_t s[2][32];
+    tmem_load_rows(s[0], mine);
+    tmem_load_rows(s[1], mine + (16u << 16));
+    // is every key of the tile there and seen by every row?
+    const int32_t v0 = (t0 + i) * kTok;
+    const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
+    const int32_t key0 = key_of(range, v0), key1 = key_of(range, v0 + kTok - 1);
+    const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu && key1 <= pos_first &&
+                     (p.window == 0 || key0 > pos_last - p.window || key1 < p.sinks);
+    const int4 ve4 = *reinterpret_cast<const int4*>(ctl.vexp[stage]);
+    const int ve[4] = {ve4.x, ve4.y, ve4.z, ve4.w};
+    const int vmax = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
+    tmem_wait_load();
+    uint64_t t[4][8];
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < kTok / 2; ++c) {
-        const float4 kp = ctl.kpar[buf][c];
-        const uint64_t acc = pair(__uint_as_float(s[c / 16][(2 * c) % 32]),
-                                  __uint_as_float(s[c / 16][(2 * c) % 32 + 1]));
-        t[c] = fma2(acc, pair(kp.x, kp.y), mul2(pair(kp.z, kp.w), qsum));
+    for (int n = 0; n < 8; ++n) {
+      const float4 kp = ctl.kpar[stage][4 * n + t4];
+      const uint64_t sk = pair(kp.x, kp.y), zk = pair(kp.z, kp.w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t acc = pair(__uint_as_float(s[k / 2][4 * n + 2 * (k % 2)]),
+                                  __uint_as_float(s[k / 2][4 * n + 2 * (k % 2) + 1]));
+        t[k][n] = fma2(acc, sk, mul2(zk, pair(qsum[k], qsum[k])));
       }
-      if (!all) {
+    }
+    if (!all) {
 #pragma unroll
-        for (int c = 0; c < kTok / 2; ++c) {
+      for (int k = 0; k < 4; ++k) {
+        const int flat = first_row + warp_row + g + 8 * k;
+        const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(flat)));
+        const int32_t pos = tok < rq.n ? rq.len - rq.n + tok : -1;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
           float x[2];
-          unpair(t[c], x[0], x[1]);
+          unpair(t[k][n], x[0], x[1]);
+          const uint32_t bits = n < 2 ? valid.x : n < 4 ? valid.y : n < 6 ? valid.z : valid.w;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int col = 2 * c + h;
+            const int col = 8 * n + 2 * t4 + h;
             const int32_t key = key_of(range, v0 + col);
-            const bool seen = ((ctl.valid[buf][col / 16] >> (2 * (col % 16))) & 1) &&
-                              key <= row.pos &&
-                              (p.window == 0 || key > row.pos - p.window || key < p.sinks);
+            const bool seen = ((bits >> (2 * (col % 16))) & 1) && key <= pos &&
+                              (p.window == 0 || key > pos - p.window || key < p.sinks);
             x[h] = seen ? x[h] : -INFINITY;
           }
-          t[c] = pair(x[0], x[1]);
+          t[k][n] = pair(x[0], x[1]);
         }
       }
-#pragma unroll
-      for (int c = 0; c < kTok / 2; ++c) {
-        float x[2];
-        unpair(t[c], x[0], x[1]);
-        top[c % 4] = fmaxf(top[c % 4], fmaxf(x[0], x[1]));
-      }
-      const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * row.a;
-      int ve[4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) ve[n] = ctl.vexp[buf][n];
-      const int vmax = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
-      const bool grow = high + static_cast<float>(vmax - row.e) - row.m > kSlack;
-      if (__any_sync(0xffffffffu, grow)) {
-        float alpha = 1.0f;
-        if (grow) {
-          const float m = fmaxf(row.m, high);
-          const int e = max(row.e, vmax);
-          const float f = exp2_approx(row.m - m);
-          row.l *= f;
-          alpha = f * pow2i(max(row.e - e, -120));
-          row.m = m;
-          row.e = e;
-        }
-        __syncwarp();
-        if (i > 0) {
-          ok = mbar_wait(&ctl.pvdone[buf ^ 1], ((i - 1) >> 1) & 1);
-          fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_load32(o, mine + L::kO + c);
-            tmem_wait_load();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_store32(mine + L::kO + c, o);
-          }
-          tmem_wait_store();
-        }
-      }
-      const uint64_t a2 = pair(row.a, row.a);
-      uint32_t pr[32];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {  // 16 tokens: one exponent of V
-        const int shift = ve[n] - row.e;
-        const float ref = static_cast<float>(shift) - row.m;
-        const uint64_t ref2 = pair(ref, ref);
-        uint64_t sum = pair(0.0f, 0.0f);
-#pragma unroll
-        for (int c = 8 * n; c < 8 * n + 8; ++c) {
-          float x[2];
-          unpair(fma2(t[c], a2, ref2), x[0], x[1]);
-          x[0] = exp2_approx(x[0]);
-          x[1] = exp2_approx(x[1]);
-          sum = add2(sum, pair(x[0], x[1]));
-          pr[c] = pack_half2(x[0], x[1]);
-        }
-        float lo, hi;
-        unpair(sum, lo, hi);
-        row.l = fmaf(lo + hi, pow2i(min(-shift, 126)), row.l);
-      }
-      tmem_store32(mine + buf * kTok, pr);
-      tmem_wait_store();
-      fence_before();
     }
-    // the rows of all four warps are written
-    __syncwarp();
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (w == 0) {
-      if (ok && lane == 0) {
-        fence_after();
-        issue_pv<D>(tmem, smem, buf, i > 0);
-        commit(&ctl.pvdone[buf]);
+    bool grow = vmax - e > kExpSlack;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        float x[2];
+        unpair(t[k][n], x[0], x[1]);
+        top[k] = fmaxf(top[k], fmaxf(x[0], x[1]));
+      }
+      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+      top[k] *= a[k];
+      grow = grow || top[k] - m[k] > kSlack;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      const int e_new = max(e, vmax);
+      const float down = pow2i(max(e - e_new, -120));
+      e = e_new;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float m_new = fmaxf(m[k], top[k]);
+        const float f = exp2_approx(m[k] - m_new);
+        m[k] = m_new;
+        l[k] *= f;
+        if (t4 == 0) ctl.alpha[warp_row + g + 8 * k] = f * down;
+      }
+      __syncwarp();
+      if (i > 0) {
+        // S of this tile is there, so the product before it has ended
+        const float alpha = ctl.alpha[warp_row + lane];
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o, mine + L::kO + c);
+          tmem_wait_load();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+          tmem_store32(mine + L::kO + c, o);
+        }
       }
       __syncwarp();
     }
+    float back[4];  // from the units of 16 tokens' P to those of l
+#pragma unroll
+    for (int n = 0; n < 4; ++n) back[n] = pow2i(min(e - ve[n], 126));
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t pr[16];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int k = 2 * half + kk;
+        const uint64_t a2 = pair(a[k], a[k]);
+        const float r = m[k] + static_cast<float>(e);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float ref = static_cast<float>(ve[n]) - r;
+          const uint64_t ref2 = pair(ref, ref);
+          float sum = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[2];
+            unpair(fma2(t[k][2 * n + h], a2, ref2), x[0], x[1]);
+            x[0] = exp2_approx(x[0]);
+            x[1] = exp2_approx(x[1]);
+            sum += x[0] + x[1];
+            pr[2 * (2 * n + h) + kk] = pack_half2(x[0], x[1]);
+          }
+          l[k] = fmaf(sum, back[n], l[k]);
+        }
+      }
+      tmem_store_rows(mine + (static_cast<uint32_t>(half) << 20), pr);
+    }
+    tmem_wait_store();
+    fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.pready[unit]);
+    if (++stage == L::kStages) stage = 0, phase ^= 1;
   }
   if (tiles > 0 && ok) {
-    ok = mbar_wait(&ctl.pvdone[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
+    ok = mbar_wait(&ctl.sready[unit], tiles & 1);  // the last product
     fence_after();
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+    if (t4 == 0) ctl.row[warp_row + g + 8 * k] = make_float2(m[k], l[k]);
+  }
+  __syncwarp();
+  e_out = e;
   return ok;
 }
 
 template <typename T, int D>
 __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq, int flat,
-                                          int kv_head, float* part, const Row& row, bool any,
-                                          uint32_t tmem) {
+                                          int kv_head, float* part, float2 ml, int e, bool any,
+                                          uint32_t mine) {
   using L = Layout<D>;
   const AttnParams& a = p.a;
-  const int w = threadIdx.x / 32;
-  const uint32_t mine = tmem + (static_cast<uint32_t>(w) << 21) + L::kO;
   const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(flat)));
   const bool there = tok < rq.n;
   const int head = kv_head * a.group + (flat - tok * a.group);
-  const float unit = pow2i(min(max(row.e, -120), 120));
-  const float f = part == nullptr ? inverse_sum(row.l) * unit : unit;
+  const float unit = pow2i(e);
+  const float f = part == nullptr ? inverse_sum(ml.y) * unit : unit;
   T* dst = static_cast<T*>(a.out) + (rq.row0 + static_cast<int64_t>(tok)) * a.out_stride +
            static_cast<int64_t>(head) * D;
 #pragma unroll 1
@@ -588,7 +677,7 @@ __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq
     uint32_t o[32];
     __syncwarp();
     if (any) {  // uniform: the whole CTA had tiles
-      tmem_load32(o, mine + c);
+      tmem_load32(o, mine + L::kO + c);
       tmem_wait_load();
     } else {
 #pragma unroll
@@ -613,11 +702,11 @@ __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq
       }
     }
   }
-  if (part != nullptr && there) *reinterpret_cast<float2*>(part) = make_float2(row.m, row.l);
+  if (part != nullptr && there) *reinterpret_cast<float2*>(part) = ml;
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(Layout<D>::kThreads, 1)
 kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   using L = Layout<D>;
   extern __shared__ uint8_t rows_smem[];
@@ -631,72 +720,77 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   pdl_launch_dependents();
   const Request rq =
       load_request(a, b, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
+  constexpr int kCtaRows = kRows * L::kUnits;
   const int64_t rows = static_cast<int64_t>(rq.n) * a.group;
-  if (static_cast<int64_t>(tile) * kRows >= rows) return;
-  const int first_row = tile * kRows;
+  if (static_cast<int64_t>(tile) * kCtaRows >= rows) return;
+  const int first_row = tile * kCtaRows;
+  const int units = rows - first_row > kRows ? L::kUnits : 1;
   const int first_tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(first_row)));
-  const int last_tok =
-      min(rq.n - 1, static_cast<int>(a.div_group.div(static_cast<uint32_t>(first_row + kRows - 1))));
+  const int last_tok = min(
+      rq.n - 1, static_cast<int>(a.div_group.div(static_cast<uint32_t>(first_row + kCtaRows - 1))));
   const int32_t pos_first = rq.len - rq.n + first_tok, pos_last = rq.len - rq.n + last_tok;
   const KeyRange range = key_range(a, pos_first, pos_last);
   const int32_t all = range.count <= 0 ? 0 : (range.count + kTok - 1) / kTok;
   const int32_t t0 = static_cast<int32_t>(static_cast<int64_t>(all) * split / p.splits);
   const int32_t t1 = static_cast<int32_t>(static_cast<int64_t>(all) * (split + 1) / p.splits);
 
-  if (warp == 0) {
+  if (warp == L::kWarps - 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&ctl.tmem)),
                  "r"(L::kColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x == 32) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&ctl.full[i], 4);
+      mbar_init(&ctl.free[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ctl.kfull[i], 4);
-      mbar_init(&ctl.vfull[i], 4);
-      mbar_init(&ctl.qkdone[i], 1);
-      mbar_init(&ctl.pvdone[i], 1);
+      mbar_init(&ctl.sready[i], 1);
+      mbar_init(&ctl.pready[i], 4);
     }
     mbar_init(&ctl.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  load_rows<T, D>(a, rq, first_row, kv_head, smem, ctl);
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  // softmax warps: this thread's row for what is done by rows
+  const int unit = warp / 4, flat = first_row + static_cast<int>(threadIdx.x);
+  const uint32_t mine = ctl.tmem + unit * L::kUnit + (static_cast<uint32_t>(warp % 4) << 21);
+  if (warp < 4 * units) {
+    load_row<T, D>(a, rq, flat, kv_head, mine + L::kQ, ctl.row[threadIdx.x]);
+  }
   fence_before();
   __syncthreads();
   fence_after();
 
-  bool ok;
-  if (warp >= 4) {
+  bool ok = true;
+  if (warp == L::kWarps - 1) {
+    ok = issue<D>(t1 - t0, units, smem_u32(smem), ctl);
+  } else if (warp >= 4 * L::kUnits) {
     ok = bring<D>(a, range, b, kv_head, t0, t1 - t0, smem, ctl);
-  } else {
-    Row row;
-    row.a = ctl.row[threadIdx.x].x;
-    row.qsum = ctl.row[threadIdx.x].y;
-    row.m = -1e30f;
-    row.l = 0.0f;
-    row.e = -100;
-    const int flat = first_row + threadIdx.x;
-    const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(flat)));
-    row.pos = tok < rq.n ? rq.len - rq.n + tok : -1;
-    ok = attend<D>(a, range, t0, t1 - t0, pos_first, pos_last, smem_u32(smem), ctl, row);
+  } else if (warp < 4 * units) {
+    int e;
+    ok = attend<D>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, unit, ctl, e);
     float* part = nullptr;
     if (p.splits > 1) {
-      const int64_t unit = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + tile;
-      part = p.part + ((unit * p.splits + split) * kRows + threadIdx.x) * (D + 4);
+      const int64_t at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + tile;
+      part = p.part + ((at * p.splits + split) * kCtaRows + threadIdx.x) * (D + 4);
     }
-    write_row<T, D>(p, rq, flat, kv_head, part, row, t1 > t0, ctl.tmem);
-    fence_before();
+    write_row<T, D>(p, rq, flat, kv_head, part, ctl.row[threadIdx.x], e, t1 > t0, mine);
   }
+  fence_before();
   if (__syncthreads_or(!ok)) {
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == L::kThreads - 32) {
       raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
       commit(&ctl.drained);  // products in flight end before their memory is given back
       mbar_wait(&ctl.drained, 0);
     }
     __syncthreads();
   }
-  if (warp == 0) {
+  if (warp == L::kWarps - 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ctl.tmem),
                  "r"(L::kColumns));
@@ -718,12 +812,14 @@ kv4_rows_join_kernel(const __grid_constant__ RowsParams p) {
   const Request rq = load_request(a, b, false);
   const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(flat)));
   if (tok >= rq.n) return;
-  const int64_t unit = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + flat / kRows;
-  const float* src = p.part + (unit * p.splits * kRows + flat % kRows) * (D + 4);
+  constexpr int kCtaRows = kRows * Layout<D>::kUnits;
+  const int64_t at =
+      (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + flat / kCtaRows;
+  const float* src = p.part + (at * p.splits * kCtaRows + flat % kCtaRows) * (D + 4);
   float m = -1e30f, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int i = 0; i < p.splits; ++i, src += kRows * (D + 4)) {
+  for (int i = 0; i < p.splits; ++i, src += kCtaRows * (D + 4)) {
     const float2 ml = *reinterpret_cast<const float2*>(src);
     const float4 v = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
     const float nm = fmaxf(m, ml.x);
@@ -744,9 +840,8 @@ kv4_rows_join_kernel(const __grid_constant__ RowsParams p) {
 
 // CTAs that share a unit: enough that few units fill the GPU, with at least
 // four tiles each.
-int split_count(int64_t units, int64_t seen, int64_t head_size) {
-  const int64_t slots = static_cast<int64_t>(current_sm_count()) * (head_size <= 128 ? 2 : 1);
-  int64_t n = slots / units;
+int split_count(int64_t units, int64_t seen) {
+  int64_t n = current_sm_count() / units;
   const int64_t most = seen / (4 * kTok);
   if (n > most) n = most;
   return static_cast<int>(n < 1 ? 1 : n);
@@ -761,23 +856,24 @@ struct RowsPlan {
 RowsPlan plan_rows(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_heads,
                    int64_t group, int64_t head_size, int64_t window, int64_t sinks) {
   RowsPlan pl;
-  pl.row_tiles = (max_query * group + kRows - 1) / kRows;
+  const int64_t cta_rows = kRows * (head_size <= 128 ? 2 : 1);
+  pl.row_tiles = (max_query * group + cta_rows - 1) / cta_rows;
   const int64_t units = batch * kv_heads * pl.row_tiles;
   int64_t seen = max_len;
-  if (window > 0 && window + sinks + kRows < seen) seen = window + sinks + kRows;
-  pl.splits = split_count(units, seen, head_size);
-  pl.part_bytes = pl.splits > 1 ? units * pl.splits * kRows * (head_size + 4) * 4 : 0;
+  if (window > 0 && window + sinks + cta_rows < seen) seen = window + sinks + cta_rows;
+  pl.splits = split_count(units, seen);
+  pl.part_bytes = pl.splits > 1 ? units * pl.splits * cta_rows * (head_size + 4) * 4 : 0;
   return pl;
 }
 
 template <typename T, int D>
 cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
-  constexpr size_t kSmem = Layout<D>::kBytes + 1024;
+  constexpr size_t kSmem = Layout<D>::kStages * Layout<D>::kStage + 1024;
   cudaError_t err = ensure_smem_limit<kv4_rows_kernel<T, D>>(kSmem, kSmem);
   if (err != cudaSuccess) return err;
   const dim3 grid(static_cast<unsigned>(p.row_tiles * p.splits),
                   static_cast<unsigned>(p.a.kv_heads), static_cast<unsigned>(p.a.batch));
-  kv4_rows_kernel<T, D><<<grid, kThreads, kSmem, stream>>>(p);
+  kv4_rows_kernel<T, D><<<grid, Layout<D>::kThreads, kSmem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1) return err;
   const int64_t rows = static_cast<int64_t>(p.a.max_query) * p.a.group;
