@@ -21,14 +21,13 @@
 // 1024 (16 a cycle), the rest of softmax and the expanding of codes about as
 // many issue slots, and shared memory as many accesses of 128 bytes; so the
 // work is laid out to keep all four going at once:
-//  - Q, as P, is read from tensor memory, and shared memory holds only K and
-//    V, up to six stages of them: four warps bring the codes from the pages and
-//    expand them (128-byte swizzle; a lane's 16-byte pieces of 4 tokens x 2
-//    halves of a panel hit all banks), far ahead of the products;
-//  - one warp issues products: while one unit computes softmax, the other's
-//    P V and next Q K^T run (P takes the place of S);
-//  - four warps a unit compute softmax. A lane has 4 rows x 16 tokens, not one
-//    row x 64 tokens, and so loads a quarter of the tokens' scales.
+//  - four warps bring the codes from the pages and expand them into a ring of
+//    stages (128-byte swizzle; a lane's 16-byte pieces of 4 tokens x 2 halves of
+//    a panel hit all banks), ahead of the products;
+//  - one warp issues products, Q K^T a tile ahead of P V, into one of two S (P,
+//    from tensor memory, takes the place of its S);
+//  - eight warps a unit compute softmax. A lane has 2 rows x 16 tokens, not one
+//    row x 32 tokens, and so loads half as many of the tokens' scales.
 // O stays in tensor memory; it is rescaled only when a row's reference grows by
 // more than 2^8, which P's range leaves room for.
 #include <climits>
@@ -45,7 +44,7 @@ constexpr int kTok = 64;    // cache tokens of a tile
 // How far P may exceed 1 before O is rescaled, log2: by a row's maximum, and
 // by the exponent of V.
 constexpr float kSlack = 8.0f;
-constexpr int kExpSlack = 4;
+constexpr float kExpSlack = 4.0f;
 
 struct RowsParams {
   AttnParams a;
@@ -53,31 +52,6 @@ struct RowsParams {
   float* part;        // [CTA's rows][splits][rows][D + 4]
   int32_t row_tiles;  // CTAs a request's rows may take
 };
-
-// Packed pairs of fp32.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 // ---------------------------------------------------------------------------
 // Tensor memory and tcgen05
@@ -135,6 +109,25 @@ __device__ __forceinline__ void tmem_store_rows(uint32_t addr, const uint32_t (&
       : "memory");
 }
 
+// The layout of the first, 32 columns.
+__device__ __forceinline__ void tmem_load_rows(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store_rows_f32(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_load() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -165,6 +158,14 @@ __host__ __device__ constexpr uint32_t instruction(int n, bool across) {
          (static_cast<uint32_t>(kRows / 16) << 24);
 }
 
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(instr), "r"(add ? 1u : 0u)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr,
                                        bool add) {
   asm volatile(
@@ -190,25 +191,33 @@ struct Layout {
   static constexpr int kPanel = kTok * 128;
   static constexpr int kV = kPanels * kPanel;      // V behind K in a stage
   static constexpr int kStage = 2 * kV;
-  static constexpr int kStages = D <= 128 ? 6 : 3;
-  static constexpr int kWarps = kUnits * 4 + 4 + 1;  // softmax, bringing, products
-  static constexpr int kThreads = kWarps * 32;
-  // Tensor memory of a unit: S (and P in its first half), Q, O.
+  static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 2;
+  static constexpr int kQPanel = kRows * 128;
+  static constexpr int kQ = kPanels * kQPanel;     // a unit's rows, in front of the stages
+  static constexpr int kBytes = kUnits * kQ + kStages * kStage;
+  // Warps: eight of softmax a unit, four that bring, one that issues products;
+  // three more fill its warpgroup. With two units the 80 registers a thread that
+  // 768 threads start with are dealt out anew by warpgroup:
+  // 16 * 96 + 4 * 64 + 4 * 32 = 24 * 80.
+  static constexpr int kBring = kUnits * 8, kIssue = kBring + 4;
+  static constexpr int kThreads = (kIssue + 4) * 32;
+  // Tensor memory of a unit: two S (P takes an S's first half), then O.
   static constexpr uint32_t kUnit = 256;
-  static constexpr uint32_t kQ = kTok;
-  static constexpr uint32_t kO = D <= 128 ? 128 : 192;
+  static constexpr uint32_t kO = 2 * kTok;
   static constexpr uint32_t kColumns = 512;
 };
 
 constexpr int kMaxStages = 6;
 
 struct Control {
-  uint64_t full[kMaxStages], free[kMaxStages], sready[2], pready[2], drained;
+  uint64_t full[kMaxStages], free[kMaxStages];
+  uint64_t sready[2][2], pready[2][2], pvdone[2];  // by unit and S
+  uint64_t drained, unused;
   float4 kpar[kMaxStages][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
   uint32_t valid[kMaxStages][4];      // two bits a token, 16 tokens each
-  int32_t vexp[kMaxStages][4];        // e of 16 tokens
+  float vexp[kMaxStages][4];          // e of 16 tokens
   float2 row[2 * kRows];              // a, sum of q 2^-24; at the end m, l
-  float alpha[2 * kRows];
+  float e[2 * kRows];                 // at the end
   uint32_t tmem;
 };
 
@@ -217,10 +226,11 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t piece) {
   return r * 128 + ((piece ^ (r & 7)) << 4);
 }
 
-// A thread's query row, scaled to fp16, into tensor memory.
+// A thread's query row, scaled to fp16, into shared memory.
 template <typename T, int D>
 __device__ __forceinline__ void load_row(const AttnParams& p, const Request& rq, int flat,
-                                         int kv_head, uint32_t q_cols, float2& factors) {
+                                         int kv_head, int r, uint8_t* smem, float2& factors) {
+  using L = Layout<D>;
   const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(flat)));
   const int head = kv_head * p.group + (flat - tok * p.group);
   const bool there = tok < rq.n;
@@ -241,29 +251,22 @@ __device__ __forceinline__ void load_row(const AttnParams& p, const Request& rq,
   // largest logit
   const float up = p.scale_log2 < 0.0f ? -pow2i(13 - e) : pow2i(13 - e);
   float sum = 0.0f;
-#pragma unroll 1
-  for (int c = 0; c < D / 2; c += 32) {
-    uint32_t q[32];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+#pragma unroll 4
+  for (int i = 0; i < D / 8; ++i) {
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (there) {
       float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-      if (there) load_query<T, 8>(src + 2 * c + 8 * i, p.q_vec != 0, x);
+      load_query<T, 8>(src + 8 * i, p.q_vec != 0, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = __half2float(__float2half_rn(x[j] * up));
         sum += x[j];
       }
-      q[4 * i] = pack_half2(x[0], x[4]);
-      q[4 * i + 1] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
-      q[4 * i + 2] = pack_half2(x[2], x[6]);
-      q[4 * i + 3] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
+      out = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1] * 0.0625f, x[5] * 0.0625f),
+                       pack_half2(x[2], x[6]), pack_half2(x[3] * 0.0625f, x[7] * 0.0625f));
     }
-    __syncwarp();
-    tmem_store32(q_cols + c, q);
+    *reinterpret_cast<uint4*>(smem + (i / 8) * L::kQPanel + swizzled(r, i % 8)) = out;
   }
-  tmem_wait_store();
   // a is never zero, so that a key that is not seen stays at -inf
   factors = make_float2(fmaxf(fabsf(p.scale_log2) * pow2i(e - 13) * 16777216.0f, 1.2e-38f),
                         sum * 5.9604645e-8f);
@@ -334,7 +337,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
                                       int kv_head, int32_t t0, int32_t tiles, uint8_t* smem,
                                       Control& ctl) {
   using L = Layout<D>;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32 - 4 * L::kUnits;
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32 - L::kBring;
   const int tok = w * 16 + lane / 2;
   const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_stride;
   const int32_t* k_head = p.cache + static_cast<int64_t>(kv_head) * (D / 8);
@@ -400,7 +403,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     }
     if (lane == 0) {
       ctl.valid[stage][w] = there;
-      ctl.vexp[stage][w] = e;
+      ctl.vexp[stage][w] = static_cast<float>(e);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -415,66 +418,65 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
 // ---------------------------------------------------------------------------
 
 template <int D>
-__device__ __forceinline__ void issue_qk(uint32_t unit, uint32_t stage) {
+__device__ __forceinline__ void issue_qk(uint32_t s, uint32_t rows, uint32_t stage) {
   using L = Layout<D>;
-  const uint64_t k = operand(stage, 0, 1024);
+  const uint64_t q = operand(rows, 0, 1024), k = operand(stage, 0, 1024);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    mma_ts(unit, unit + L::kQ + i * 8, k + (((i / 4) * L::kPanel + (i % 4) * 32) >> 4),
-           instruction(kTok, false), i > 0);
+    mma_ss(s, q + (((i / 4) * L::kQPanel + (i % 4) * 32) >> 4),
+           k + (((i / 4) * L::kPanel + (i % 4) * 32) >> 4), instruction(kTok, false), i > 0);
   }
 }
 
 template <int D>
-__device__ __forceinline__ void issue_pv(uint32_t unit, uint32_t stage, bool add) {
+__device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t stage, bool add) {
   using L = Layout<D>;
   const uint64_t v = operand(stage + L::kV, L::kPanel, 1024);
 #pragma unroll
   for (int i = 0; i < kTok / 16; ++i) {
-    mma_ts(unit + L::kO, unit + i * 8, v + ((i * 16 * 128) >> 4), instruction(D, true),
-           add || i > 0);
+    mma_ts(o, p + i * 8, v + ((i * 16 * 128) >> 4), instruction(D, true), add || i > 0);
   }
 }
 
+// Q K^T runs a tile ahead of P V: softmax finds the next S when it is done with
+// one.
 template <int D>
 __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, Control& ctl) {
   using L = Layout<D>;
-  if (tiles == 0) return true;
   const bool leader = threadIdx.x % 32 == 0;
-  const uint32_t tmem = ctl.tmem;
-  if (!mbar_wait(&ctl.full[0], 0)) return false;
-  fence_after();
-  if (leader) {
-    for (int u = 0; u < units; ++u) {
-      issue_qk<D>(tmem + u * L::kUnit, smem);
-      commit(&ctl.sready[u]);
-    }
-  }
-  __syncwarp();
-  int stage = 0;
-  uint32_t phase = 0;
-  for (int32_t i = 0; i < tiles; ++i) {
-    const int next = stage + 1 == L::kStages ? 0 : stage + 1;
-    const uint32_t next_phase = stage + 1 == L::kStages ? phase ^ 1 : phase;
-    for (int u = 0; u < units; ++u) {
-      const uint32_t unit = tmem + u * L::kUnit;
-      if (!mbar_wait(&ctl.pready[u], i & 1)) return false;
+  const uint32_t tmem = ctl.tmem, stages = smem + L::kUnits * L::kQ;
+  int stage = 0, qk_stage = 0;
+  uint32_t qk_phase = 0;
+  for (int32_t i = -1; i < tiles; ++i) {
+    if (i + 1 < tiles) {
+      if (!mbar_wait(&ctl.full[qk_stage], qk_phase)) return false;
       fence_after();
       if (leader) {
-        issue_pv<D>(unit, smem + stage * L::kStage, i > 0);
+        const int buf = (i + 1) & 1;
+        for (int u = 0; u < units; ++u) {
+          // into the S whose P the product of tile i - 1 reads: products run in order
+          issue_qk<D>(tmem + u * L::kUnit + buf * kTok, smem + u * L::kQ,
+                      stages + qk_stage * L::kStage);
+          commit(&ctl.sready[u][buf]);
+        }
+      }
+      __syncwarp();
+      if (++qk_stage == L::kStages) qk_stage = 0, qk_phase ^= 1;
+    }
+    if (i < 0) continue;
+    const int buf = i & 1;
+    for (int u = 0; u < units; ++u) {
+      if (!mbar_wait(&ctl.pready[u][buf], (i >> 1) & 1)) return false;
+      fence_after();
+      if (leader) {
+        const uint32_t unit = tmem + u * L::kUnit;
+        issue_pv<D>(unit + L::kO, unit + buf * kTok, stages + stage * L::kStage, i > 0);
+        commit(&ctl.pvdone[u]);
         if (u == units - 1) commit(&ctl.free[stage]);
       }
       __syncwarp();
-      if (i + 1 < tiles) {
-        if (u == 0 && !mbar_wait(&ctl.full[next], next_phase)) return false;
-        // into the S whose P the product before reads: products run in order
-        if (leader) issue_qk<D>(unit, smem + next * L::kStage);
-      }
-      if (leader) commit(&ctl.sready[u]);
-      __syncwarp();
     }
-    stage = next;
-    phase = next_phase;
+    if (++stage == L::kStages) stage = 0;
   }
   return true;
 }
@@ -483,197 +485,201 @@ __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, C
 // The warps that have the query rows
 // ---------------------------------------------------------------------------
 
-// Lane (g, t) has rows g + 8 k of the warp's 32, k < 4, and of each the tokens
-// 8 n + 2 t and 8 n + 2 t + 1 of a tile. A row's reference m (log2) and its sum
-// l, in units of 2^m; O is in units of 2^(m + e), e the same for all rows of a
-// warp.
+// A thread's part of a tile: lane (g, t) has rows g and g + 8 of its warp's 16,
+// and of each the tokens 8 n + 2 t and 8 n + 2 t + 1.
+struct Part {
+  float a[2], qsum[2];  // rows' factors
+  float m[2];           // references (log2)
+  float top[2];         // largest t of this tile
+  float l[2];           // sums of this tile, in units of 2^m
+  int32_t hi[2];        // last key seen, as a virtual token
+};
+
+// S into P and the rows' largest t and sums. `ve` are the exponents of V's 16
+// tokens each, `e` the warp's.
+template <bool kAll>
+__device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_cols,
+                                             const float4* kpar, const uint32_t* valid,
+                                             const float* vexp, int32_t v0, float e, Part& part,
+                                             uint32_t (&pr)[16]) {
+  const int t4 = threadIdx.x % 4;
+  uint32_t s[32];
+  tmem_load_rows(s, s_cols);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) part.top[k] = -INFINITY, part.l[k] = 0.0f;
+  tmem_wait_load();
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {  // 16 tokens: one exponent of V
+    const float ve = vexp[n], back = exp2_approx(e - ve);  // to the units of l
+    const float4 kp[2] = {kpar[8 * n + t4], kpar[8 * n + 4 + t4]};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float ref = ve - (part.m[k] + e);
+      float t[4], x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 f = kp[j / 2];
+        t[j] = fmaf(__uint_as_float(s[8 * n + 4 * (j / 2) + 2 * k + j % 2]), j % 2 ? f.y : f.x,
+                    (j % 2 ? f.w : f.z) * part.qsum[k]);
+        if constexpr (!kAll) {
+          const int col = 16 * n + 8 * (j / 2) + 2 * t4 + j % 2, v = v0 + col;
+          const bool seen = v <= part.hi[k] &&
+                            (p.window == 0 || v > part.hi[k] - p.window || v < p.sinks) &&
+                            ((valid[n] >> (2 * (col % 16))) & 1);
+          t[j] = seen ? t[j] : -INFINITY;
+        }
+        x[j] = exp2_approx(fmaf(t[j], part.a[k], ref));
+      }
+      part.top[k] = fmaxf(part.top[k], fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+      part.l[k] = fmaf((x[0] + x[1]) + (x[2] + x[3]), back, part.l[k]);
+      pr[4 * n + k] = pack_half2(x[0], x[1]);
+      pr[4 * n + 2 + k] = pack_half2(x[2], x[3]);
+    }
+  }
+}
+
+// A warp has 16 of a unit's rows: warps w and w + 4 have those of tensor memory
+// lanes 32 w ..., 16 each. Sums l are in units of 2^m, O in units of 2^(m + e),
+// e the same for all rows of a warp. P is taken with the references that are
+// there; only a tile that outgrows them by the slack (the first one, and few
+// after it) is taken again, with new ones. So nothing waits for a tile's
+// maximum, and a thread never holds more than the tile's S.
 template <int D>
 __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& range, int32_t t0,
                                        int32_t tiles, int32_t pos_first, int32_t pos_last,
-                                       const Request& rq, int first_row, int unit, Control& ctl,
-                                       int& e_out) {
+                                       const Request& rq, int first_row, Control& ctl) {
   using L = Layout<D>;
+  const int warp = threadIdx.x / 32, unit = warp / 8;
   const int lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-  const int warp_row = unit * kRows + (threadIdx.x / 32 % 4) * 32;  // of the CTA's rows
-  const uint32_t mine = ctl.tmem + unit * L::kUnit +
-                        (static_cast<uint32_t>(threadIdx.x / 32 % 4) << 21);
-  float a[4], m[4], l[4];
-  float qsum[4];
+  const int lanes = (warp % 4) * 32 + (warp / 4 % 2) * 16;  // of tensor memory
+  const int warp_row = unit * kRows + lanes;                // of the CTA's rows
+  const uint32_t mine = ctl.tmem + unit * L::kUnit + (static_cast<uint32_t>(lanes) << 16);
+  // Visible keys of a row at position i, as virtual tokens (KeyRange): v <= hi,
+  // and with a window v > hi - window or v < sinks.
+  const int32_t to_v = range.head - range.first;
+  const int32_t hi_first = pos_first + to_v, hi_last = pos_last + to_v;
+  Part part;
+  float l[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = ctl.row[warp_row + g + 8 * k];
-    a[k] = f.x;
-    qsum[k] = f.y;
-    m[k] = -1e30f;
+  for (int k = 0; k < 2; ++k) {
+    const int row = warp_row + g + 8 * k;
+    const float2 f = ctl.row[row];
+    part.a[k] = f.x;
+    part.qsum[k] = f.y;
+    part.m[k] = -1e30f;
     l[k] = 0.0f;
+    const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(first_row + row)));
+    part.hi[k] = tok < rq.n ? rq.len - rq.n + tok + to_v : -1;
   }
-  int e = -100;
+  float e = -100.0f;
   bool ok = true;
   int stage = 0;
   uint32_t phase = 0;
   for (int32_t i = 0; i < tiles; ++i) {
-    if (!mbar_wait(&ctl.full[stage], phase) || !mbar_wait(&ctl.sready[unit], i & 1)) {
+    if (!mbar_wait(&ctl.full[stage], phase) ||
+        !mbar_wait(&ctl.sready[unit][i & 1], (i >> 1) & 1)) {
       ok = false;
       break;
     }
     fence_after();
-    uint32_t s[2][32];
-    tmem_load_rows(s[0], mine);
-    tmem_load_rows(s[1], mine + (16u << 16));
+    const uint32_t s_cols = mine + (i & 1) * kTok;
     // is every key of the tile there and seen by every row?
     const int32_t v0 = (t0 + i) * kTok;
-    const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
-    const int32_t key0 = key_of(range, v0), key1 = key_of(range, v0 + kTok - 1);
-    const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu && key1 <= pos_first &&
-                     (p.window == 0 || key0 > pos_last - p.window || key1 < p.sinks);
-    const int4 ve4 = *reinterpret_cast<const int4*>(ctl.vexp[stage]);
-    const int ve[4] = {ve4.x, ve4.y, ve4.z, ve4.w};
-    const int vmax = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
-    tmem_wait_load();
-    uint64_t t[4][8];
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float4 kp = ctl.kpar[stage][4 * n + t4];
-      const uint64_t sk = pair(kp.x, kp.y), zk = pair(kp.z, kp.w);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint64_t acc = pair(__uint_as_float(s[k / 2][4 * n + 2 * (k % 2)]),
-                                  __uint_as_float(s[k / 2][4 * n + 2 * (k % 2) + 1]));
-        t[k][n] = fma2(acc, sk, mul2(zk, pair(qsum[k], qsum[k])));
-      }
+    bool all;
+    float vmax;
+    {
+      const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
+      all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu && v0 + kTok - 1 <= hi_first &&
+            (p.window == 0 || v0 > hi_last - p.window || v0 + kTok - 1 < p.sinks);
+      const float4 ve = *reinterpret_cast<const float4*>(ctl.vexp[stage]);
+      vmax = fmaxf(fmaxf(ve.x, ve.y), fmaxf(ve.z, ve.w));
     }
-    if (!all) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int flat = first_row + warp_row + g + 8 * k;
-        const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(flat)));
-        const int32_t pos = tok < rq.n ? rq.len - rq.n + tok : -1;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          float x[2];
-          unpair(t[k][n], x[0], x[1]);
-          const uint32_t bits = n < 2 ? valid.x : n < 4 ? valid.y : n < 6 ? valid.z : valid.w;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = 8 * n + 2 * t4 + h;
-            const int32_t key = key_of(range, v0 + col);
-            const bool seen = ((bits >> (2 * (col % 16))) & 1) && key <= pos &&
-                              (p.window == 0 || key > pos - p.window || key < p.sinks);
-            x[h] = seen ? x[h] : -INFINITY;
-          }
-          t[k][n] = pair(x[0], x[1]);
-        }
+    uint32_t pr[16];
+    for (;;) {
+      if (all) {
+        softmax_tile<true>(p, s_cols, ctl.kpar[stage], ctl.valid[stage], ctl.vexp[stage], v0, e,
+                           part, pr);
+      } else {
+        softmax_tile<false>(p, s_cols, ctl.kpar[stage], ctl.valid[stage], ctl.vexp[stage], v0, e,
+                            part, pr);
       }
-    }
-    bool grow = vmax - e > kExpSlack;
+      bool grow = vmax - e > kExpSlack;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        float x[2];
-        unpair(t[k][n], x[0], x[1]);
-        top[k] = fmaxf(top[k], fmaxf(x[0], x[1]));
+      for (int k = 0; k < 2; ++k) {
+        part.top[k] *= part.a[k];
+        grow = grow || part.top[k] - part.m[k] > kSlack;
       }
-      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-      top[k] *= a[k];
-      grow = grow || top[k] - m[k] > kSlack;
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-      const int e_new = max(e, vmax);
-      const float down = pow2i(max(e - e_new, -120));
+      if (!__any_sync(0xffffffffu, grow)) break;
+      const float e_new = fmaxf(e, vmax);
+      const float down = exp2_approx(e - e_new);
       e = e_new;
+      float alpha[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float m_new = fmaxf(m[k], top[k]);
-        const float f = exp2_approx(m[k] - m_new);
-        m[k] = m_new;
+      for (int k = 0; k < 2; ++k) {
+        part.top[k] = fmaxf(part.top[k], __shfl_xor_sync(0xffffffffu, part.top[k], 1));
+        part.top[k] = fmaxf(part.top[k], __shfl_xor_sync(0xffffffffu, part.top[k], 2));
+        const float m_new = fmaxf(part.m[k], part.top[k]);
+        const float f = exp2_approx(part.m[k] - m_new);
+        part.m[k] = m_new;
         l[k] *= f;
-        if (t4 == 0) ctl.alpha[warp_row + g + 8 * k] = f * down;
+        alpha[k] = f * down;
       }
-      __syncwarp();
       if (i > 0) {
-        // S of this tile is there, so the product before it has ended
-        const float alpha = ctl.alpha[warp_row + lane];
+        ok = mbar_wait(&ctl.pvdone[unit], (i - 1) & 1) && ok;
+        fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o, mine + L::kO + c);
+          uint32_t o[16];
+          tmem_load_rows(o, mine + L::kO + c);
           tmem_wait_load();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-          tmem_store32(mine + L::kO + c, o);
-        }
-      }
-      __syncwarp();
-    }
-    float back[4];  // from the units of 16 tokens' P to those of l
-#pragma unroll
-    for (int n = 0; n < 4; ++n) back[n] = pow2i(min(e - ve[n], 126));
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t pr[16];
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int k = 2 * half + kk;
-        const uint64_t a2 = pair(a[k], a[k]);
-        const float r = m[k] + static_cast<float>(e);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float ref = static_cast<float>(ve[n]) - r;
-          const uint64_t ref2 = pair(ref, ref);
-          float sum = 0.0f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[2];
-            unpair(fma2(t[k][2 * n + h], a2, ref2), x[0], x[1]);
-            x[0] = exp2_approx(x[0]);
-            x[1] = exp2_approx(x[1]);
-            sum += x[0] + x[1];
-            pr[2 * (2 * n + h) + kk] = pack_half2(x[0], x[1]);
+          for (int j = 0; j < 16; ++j) {
+            o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha[j / 2 % 2]);
           }
-          l[k] = fmaf(sum, back[n], l[k]);
+          tmem_store_rows_f32(mine + L::kO + c, o);
         }
       }
-      tmem_store_rows(mine + (static_cast<uint32_t>(half) << 20), pr);
     }
+    tmem_store_rows(s_cols, pr);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) l[k] += part.l[k];
     tmem_wait_store();
     fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.pready[unit]);
+    if (lane == 0) mbar_arrive(&ctl.pready[unit][i & 1]);
     if (++stage == L::kStages) stage = 0, phase ^= 1;
   }
   if (tiles > 0 && ok) {
-    ok = mbar_wait(&ctl.sready[unit], tiles & 1);  // the last product
+    ok = mbar_wait(&ctl.pvdone[unit], (tiles - 1) & 1);  // the last product
     fence_after();
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
     l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
     l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
-    if (t4 == 0) ctl.row[warp_row + g + 8 * k] = make_float2(m[k], l[k]);
+    if (t4 == 0) {
+      ctl.row[warp_row + g + 8 * k] = make_float2(part.m[k], l[k]);
+      ctl.e[warp_row + g + 8 * k] = e;
+    }
   }
-  __syncwarp();
-  e_out = e;
   return ok;
 }
 
 template <typename T, int D>
 __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq, int flat,
-                                          int kv_head, float* part, float2 ml, int e, bool any,
-                                          uint32_t mine) {
+                                          int kv_head, float* part, float2 ml, float e, bool any,
+                                          uint32_t mine, int c0, int c1) {
   using L = Layout<D>;
   const AttnParams& a = p.a;
   const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(flat)));
   const bool there = tok < rq.n;
   const int head = kv_head * a.group + (flat - tok * a.group);
-  const float unit = pow2i(e);
+  const float unit = exp2_approx(e);
   const float f = part == nullptr ? inverse_sum(ml.y) * unit : unit;
   T* dst = static_cast<T*>(a.out) + (rq.row0 + static_cast<int64_t>(tok)) * a.out_stride +
            static_cast<int64_t>(head) * D;
 #pragma unroll 1
-  for (int c = 0; c < D; c += 32) {
+  for (int c = c0; c < c1; c += 32) {
     uint32_t o[32];
     __syncwarp();
     if (any) {  // uniform: the whole CTA had tiles
@@ -702,7 +708,7 @@ __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq
       }
     }
   }
-  if (part != nullptr && there) *reinterpret_cast<float2*>(part) = ml;
+  if (part != nullptr && there && c0 == 0) *reinterpret_cast<float2*>(part) = ml;
 }
 
 template <typename T, int D>
@@ -734,7 +740,7 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   const int32_t t0 = static_cast<int32_t>(static_cast<int64_t>(all) * split / p.splits);
   const int32_t t1 = static_cast<int32_t>(static_cast<int64_t>(all) * (split + 1) / p.splits);
 
-  if (warp == L::kWarps - 1) {
+  if (warp == L::kIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&ctl.tmem)),
                  "r"(L::kColumns)
@@ -747,8 +753,11 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
       mbar_init(&ctl.free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ctl.sready[i], 1);
-      mbar_init(&ctl.pready[i], 4);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&ctl.sready[i][j], 1);
+        mbar_init(&ctl.pready[i][j], 8);
+      }
+      mbar_init(&ctl.pvdone[i], 1);
     }
     mbar_init(&ctl.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -756,41 +765,49 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   fence_before();
   __syncthreads();
   fence_after();
-  // softmax warps: this thread's row for what is done by rows
-  const int unit = warp / 4, flat = first_row + static_cast<int>(threadIdx.x);
+  // softmax warps: this thread's row and half of the columns for what is done
+  // by rows
+  const int unit = warp / 8, side = warp / 4 % 2;
+  const int cta_row = unit * kRows + threadIdx.x % kRows, flat = first_row + cta_row;
   const uint32_t mine = ctl.tmem + unit * L::kUnit + (static_cast<uint32_t>(warp % 4) << 21);
-  if (warp < 4 * units) {
-    load_row<T, D>(a, rq, flat, kv_head, mine + L::kQ, ctl.row[threadIdx.x]);
+  if (warp < 8 * units && side == 0) {
+    load_row<T, D>(a, rq, flat, kv_head, threadIdx.x % kRows, smem + unit * L::kQ,
+                   ctl.row[cta_row]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   fence_before();
   __syncthreads();
   fence_after();
 
   bool ok = true;
-  if (warp == L::kWarps - 1) {
-    ok = issue<D>(t1 - t0, units, smem_u32(smem), ctl);
-  } else if (warp >= 4 * L::kUnits) {
-    ok = bring<D>(a, range, b, kv_head, t0, t1 - t0, smem, ctl);
-  } else if (warp < 4 * units) {
-    int e;
-    ok = attend<D>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, unit, ctl, e);
+  if (warp >= L::kIssue) {
+    if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp == L::kIssue) ok = issue<D>(t1 - t0, units, smem_u32(smem), ctl);
+  } else if (warp >= L::kBring) {
+    if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    ok = bring<D>(a, range, b, kv_head, t0, t1 - t0, smem + L::kUnits * L::kQ, ctl);
+  } else if (warp < 8 * units) {
+    if (L::kUnits == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    ok = attend<D>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, ctl);
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + unit) : "memory");  // the unit's rows are done
     float* part = nullptr;
     if (p.splits > 1) {
       const int64_t at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + tile;
-      part = p.part + ((at * p.splits + split) * kCtaRows + threadIdx.x) * (D + 4);
+      part = p.part + ((at * p.splits + split) * kCtaRows + cta_row) * (D + 4);
     }
-    write_row<T, D>(p, rq, flat, kv_head, part, ctl.row[threadIdx.x], e, t1 > t0, mine);
+    write_row<T, D>(p, rq, flat, kv_head, part, ctl.row[cta_row], ctl.e[cta_row], t1 > t0, mine,
+                    side * (D / 2), (side + 1) * (D / 2));
   }
   fence_before();
   if (__syncthreads_or(!ok)) {
-    if (threadIdx.x == L::kThreads - 32) {
+    if (threadIdx.x == L::kIssue * 32) {
       raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
       commit(&ctl.drained);  // products in flight end before their memory is given back
       mbar_wait(&ctl.drained, 0);
     }
     __syncthreads();
   }
-  if (warp == L::kWarps - 1) {
+  if (warp == L::kIssue) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ctl.tmem),
                  "r"(L::kColumns));
@@ -868,7 +885,7 @@ RowsPlan plan_rows(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv
 
 template <typename T, int D>
 cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
-  constexpr size_t kSmem = Layout<D>::kStages * Layout<D>::kStage + 1024;
+  constexpr size_t kSmem = Layout<D>::kBytes + 1024;
   cudaError_t err = ensure_smem_limit<kv4_rows_kernel<T, D>>(kSmem, kSmem);
   if (err != cudaSuccess) return err;
   const dim3 grid(static_cast<unsigned>(p.row_tiles * p.splits),
