@@ -141,14 +141,27 @@ __device__ __forceinline__ void fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// True in one lane of a converged warp. The compiler knows that what such a
+// branch guards runs in one thread, and issues its products without asking
+// again for each of them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // Shared-memory operand descriptor: 128-byte swizzle (8 rows of 128 bytes),
-// `stride` bytes from one group of 8 rows to the next and `lead` bytes from one
-// 64-element panel to the next (operands whose rows run along K).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3fff) |
-         (static_cast<uint64_t>((lead >> 4) & 0x3fff) << 16) |
-         (static_cast<uint64_t>((stride >> 4) & 0x3fff) << 32) | (uint64_t{1} << 46) |
-         (uint64_t{2} << 61);
+// 1024 bytes from one group of 8 rows to the next and `lead` bytes from one
+// 64-element panel to the next (operands whose rows run along K). The low word
+// holds the address and `lead`; adding bytes / 16 to it moves the operand.
+__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t lead) {
+  return ((addr >> 4) & 0x3fff) | (((lead >> 4) & 0x3fff) << 16);
+}
+__device__ __forceinline__ uint64_t operand(uint32_t low) {
+  constexpr uint32_t kHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+  return static_cast<uint64_t>(low) | (static_cast<uint64_t>(kHigh) << 32);
 }
 
 // fp16 x fp16 into fp32, M = 128; `across`: B's rows run along K (V as it is
@@ -420,21 +433,21 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
 template <int D>
 __device__ __forceinline__ void issue_qk(uint32_t s, uint32_t rows, uint32_t stage) {
   using L = Layout<D>;
-  const uint64_t q = operand(rows, 0, 1024), k = operand(stage, 0, 1024);
+  const uint32_t q = operand_low(rows, 0), k = operand_low(stage, 0);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    mma_ss(s, q + (((i / 4) * L::kQPanel + (i % 4) * 32) >> 4),
-           k + (((i / 4) * L::kPanel + (i % 4) * 32) >> 4), instruction(kTok, false), i > 0);
+    mma_ss(s, operand(q + ((i / 4) * L::kQPanel + (i % 4) * 32) / 16),
+           operand(k + ((i / 4) * L::kPanel + (i % 4) * 32) / 16), instruction(kTok, false), i > 0);
   }
 }
 
 template <int D>
 __device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t stage, bool add) {
   using L = Layout<D>;
-  const uint64_t v = operand(stage + L::kV, L::kPanel, 1024);
+  const uint32_t v = operand_low(stage + L::kV, L::kPanel);
 #pragma unroll
   for (int i = 0; i < kTok / 16; ++i) {
-    mma_ts(o, p + i * 8, v + ((i * 16 * 128) >> 4), instruction(D, true), add || i > 0);
+    mma_ts(o, p + i * 8, operand(v + i * 16 * 128 / 16), instruction(D, true), add || i > 0);
   }
 }
 
@@ -443,7 +456,6 @@ __device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t stage,
 template <int D>
 __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, Control& ctl) {
   using L = Layout<D>;
-  const bool leader = threadIdx.x % 32 == 0;
   const uint32_t tmem = ctl.tmem, stages = smem + L::kUnits * L::kQ;
   int stage = 0, qk_stage = 0;
   uint32_t qk_phase = 0;
@@ -451,7 +463,7 @@ __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, C
     if (i + 1 < tiles) {
       if (!mbar_wait(&ctl.full[qk_stage], qk_phase)) return false;
       fence_after();
-      if (leader) {
+      if (elect_one()) {
         const int buf = (i + 1) & 1;
         for (int u = 0; u < units; ++u) {
           // into the S whose P the product of tile i - 1 reads: products run in order
@@ -468,7 +480,7 @@ __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, C
     for (int u = 0; u < units; ++u) {
       if (!mbar_wait(&ctl.pready[u][buf], (i >> 1) & 1)) return false;
       fence_after();
-      if (leader) {
+      if (elect_one()) {
         const uint32_t unit = tmem + u * L::kUnit;
         issue_pv<D>(unit + L::kO, unit + buf * kTok, stages + stage * L::kStage, i > 0);
         commit(&ctl.pvdone[u]);
