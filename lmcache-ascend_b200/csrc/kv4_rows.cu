@@ -53,6 +53,33 @@ struct RowsParams {
   int32_t row_tiles;  // CTAs a request's rows may take
 };
 
+// Packed pairs of fp32: one instruction for two values.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
 // Tensor memory and tcgen05
 // ---------------------------------------------------------------------------
@@ -228,7 +255,7 @@ struct Control {
   uint64_t drained, unused;
   float4 kpar[kMaxStages][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
   uint32_t valid[kMaxStages][4];      // two bits a token, 16 tokens each
-  float vexp[kMaxStages][4];          // e of 16 tokens
+  float2 vexp[kMaxStages][4];         // e of 16 tokens, twice
   float2 row[2 * kRows];              // a, sum of q 2^-24; at the end m, l
   float e[2 * kRows];                 // at the end
   uint32_t tmem;
@@ -298,6 +325,20 @@ struct Codes {
   bool there;
 };
 
+// Loads that stay where they are written: a tile ahead of their use.
+__device__ __forceinline__ uint4 load_ahead4(const int32_t* src) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(src));
+  return v;
+}
+__device__ __forceinline__ uint32_t load_ahead(const int32_t* src) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(src));
+  return v;
+}
+
 template <int D>
 __device__ __forceinline__ void fetch(const AttnParams& p, const int32_t* k_head,
                                       const int32_t* par, int32_t row, int lane, Codes<D>& c) {
@@ -308,11 +349,11 @@ __device__ __forceinline__ void fetch(const AttnParams& p, const int32_t* k_head
     const int32_t* v = k + p.half_words;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-      c.k[i] = __ldg(reinterpret_cast<const uint4*>(k + 8 * i));
-      c.v[i] = __ldg(reinterpret_cast<const uint4*>(v + 8 * i));
+      c.k[i] = load_ahead4(k + 8 * i);
+      c.v[i] = load_ahead4(v + 8 * i);
     }
-    c.kpar = static_cast<uint32_t>(__ldg(par + at));
-    c.vpar = static_cast<uint32_t>(__ldg(par + p.half_words + at));
+    c.kpar = load_ahead(par + at);
+    c.vpar = load_ahead(par + p.half_words + at);
   } else {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) c.k[i] = c.v[i] = make_uint4(0, 0, 0, 0);
@@ -327,17 +368,15 @@ __device__ __forceinline__ __half2 as_half2(uint32_t v) {
   return *reinterpret_cast<const __half2*>(&v);
 }
 
-// Eight values of V in the order 0, 4, 1, 5, 2, 6, 3, 7: codes on top of 1024,
-// which comes off exactly, times s, plus z, rounded once.
-__device__ __forceinline__ uint4 expand_v(uint32_t w, __half2 s, __half2 z) {
-  const __half2 base = __half2half2(__ushort_as_half(0x6400));
-  uint32_t r[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const __half2 c = __hsub2(as_half2(((w >> (4 * j)) & 0x000f000fu) | 0x64006400u), base);
-    r[j] = half2_bits(__hfma2(c, s, z));
-  }
-  return make_uint4(r[0], r[1], r[2], r[3]);
+// Eight values of V in the order 0, 4, 1, 5, 2, 6, 3, 7, of the bit patterns that
+// expand_k makes: c 2^-24 times s 2^24 (or 16 c 2^-24 times s 2^20), plus z,
+// rounded once.
+__device__ __forceinline__ uint4 expand_v(uint32_t w, __half2 s24, __half2 s20, __half2 z) {
+  const uint32_t x = w >> 8;
+  return make_uint4(half2_bits(__hfma2(as_half2(w & 0x000f000fu), s24, z)),
+                    half2_bits(__hfma2(as_half2(w & 0x00f000f0u), s20, z)),
+                    half2_bits(__hfma2(as_half2(x & 0x000f000fu), s24, z)),
+                    half2_bits(__hfma2(as_half2(x & 0x00f000f0u), s20, z)));
 }
 
 __device__ __forceinline__ uint4 expand_k(uint32_t w) {
@@ -361,7 +400,8 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
   const auto page_of = [&](int32_t i) {
     const int32_t v = (t0 + i) * kTok + tok;
     if (i >= tiles || v >= range.count) return -1;
-    return __ldg(table + p.div_block.div(static_cast<uint32_t>(key_of(range, v))));
+    return static_cast<int32_t>(
+        load_ahead(table + p.div_block.div(static_cast<uint32_t>(key_of(range, v)))));
   };
   const auto row_in = [&](int32_t i, int32_t page) {
     const int32_t v = (t0 + i) * kTok + tok;
@@ -386,13 +426,16 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     const Codes<D> c = next;
     fetch<D>(p, k_head, par, row_in(i + 1, page), lane, next);
     page = page_of(i + 2);
-    // the exponent above the largest value of these 16 tokens
+    // The exponent 8 above the largest value of these 16 tokens: a value's span
+    // is below 2^-7 then, s 2^24 below 2^14. What is lost, with the smallest
+    // values of the 16, is 2^-17 of the largest.
     const float s = half_lo(c.vpar), z = half_hi(c.vpar);
     const float most = fmaxf(fabsf(z), fabsf(fmaf(15.0f, s, z)));
     const int e = static_cast<int>(__reduce_max_sync(
-                      0xffffffffu, max((__float_as_uint(most) >> 23) & 255u, 80u))) - 126;
+                      0xffffffffu, max((__float_as_uint(most) >> 23) & 255u, 80u))) - 118;
     const float down = pow2i(-e);
-    const __half2 s2 = __half2half2(__float2half_rn(s * down));
+    const __half2 s24 = __half2half2(__float2half_rn(s * down * 16777216.0f));
+    const __half2 s20 = __half2half2(__float2half_rn(s * down * 1048576.0f));
     const __half2 z2 = __half2half2(__float2half_rn(z * down));
     const uint32_t there = __ballot_sync(0xffffffffu, c.there);
     if (i >= L::kStages && !mbar_wait(&ctl.free[stage], phase)) return false;
@@ -406,7 +449,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
       for (int j = 0; j < 4; ++j) {
         uint8_t* to = k + n * L::kPanel + swizzled(tok, piece + j);
         *reinterpret_cast<uint4*>(to) = expand_k(kw[j]);
-        *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], s2, z2);
+        *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], s24, s20, z2);
       }
     }
     if (lane % 2 == 0) {
@@ -416,7 +459,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     }
     if (lane == 0) {
       ctl.valid[stage][w] = there;
-      ctl.vexp[stage][w] = static_cast<float>(e);
+      ctl.vexp[stage][w] = make_float2(static_cast<float>(e), static_cast<float>(e));
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -500,7 +543,8 @@ __device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, C
 // A thread's part of a tile: lane (g, t) has rows g and g + 8 of its warp's 16,
 // and of each the tokens 8 n + 2 t and 8 n + 2 t + 1.
 struct Part {
-  float a[2], qsum[2];  // rows' factors
+  float a[2];
+  uint64_t qsum[2];     // rows' factors, the second twice
   float m[2];           // references (log2)
   float top[2];         // largest t of this tile
   float l[2];           // sums of this tile, in units of 2^m
@@ -511,43 +555,61 @@ struct Part {
 // tokens each, `e` the warp's.
 template <bool kAll>
 __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_cols,
-                                             const float4* kpar, const uint32_t* valid,
-                                             const float* vexp, int32_t v0, float e, Part& part,
+                                             const ulonglong2* kpar, const uint32_t* valid,
+                                             const float2* vexp, int32_t v0, float e, Part& part,
                                              uint32_t (&pr)[16]) {
   const int t4 = threadIdx.x % 4;
   uint32_t s[32];
   tmem_load_rows(s, s_cols);
+  uint64_t back_ref[2], a2[2];
+  float top[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) part.top[k] = -INFINITY, part.l[k] = 0.0f;
+  for (int k = 0; k < 2; ++k) {
+    const float r = -(part.m[k] + e);
+    back_ref[k] = pair(r, r);
+    a2[k] = pair(part.a[k], part.a[k]);
+    top[k] = -INFINITY;
+    part.l[k] = 0.0f;
+  }
   tmem_wait_load();
 #pragma unroll
   for (int n = 0; n < 4; ++n) {  // 16 tokens: one exponent of V
-    const float ve = vexp[n], back = exp2_approx(e - ve);  // to the units of l
-    const float4 kp[2] = {kpar[8 * n + t4], kpar[8 * n + 4 + t4]};
+    const uint64_t ve = *reinterpret_cast<const uint64_t*>(&vexp[n]);
+    const float back = exp2_approx(e - unpair(ve).x);  // to the units of l
+    const ulonglong2 kp[2] = {kpar[8 * n + t4], kpar[8 * n + 4 + t4]};  // (sk, sk), (zk, zk)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float ref = ve - (part.m[k] + e);
-      float t[4], x[4];
+      const uint64_t ref = add2(ve, back_ref[k]);
+      float2 x[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 f = kp[j / 2];
-        t[j] = fmaf(__uint_as_float(s[8 * n + 4 * (j / 2) + 2 * k + j % 2]), j % 2 ? f.y : f.x,
-                    (j % 2 ? f.w : f.z) * part.qsum[k]);
+      for (int h = 0; h < 2; ++h) {
+        const int at = 8 * n + 4 * h + 2 * k;
+        uint64_t t2 = fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), kp[h].x,
+                           mul2(kp[h].y, part.qsum[k]));
+        float2 t = unpair(t2);
         if constexpr (!kAll) {
-          const int col = 16 * n + 8 * (j / 2) + 2 * t4 + j % 2, v = v0 + col;
-          const bool seen = v <= part.hi[k] &&
-                            (p.window == 0 || v > part.hi[k] - p.window || v < p.sinks) &&
-                            ((valid[n] >> (2 * (col % 16))) & 1);
-          t[j] = seen ? t[j] : -INFINITY;
+          const int col = 16 * n + 8 * h + 2 * t4, v = v0 + col;
+          const uint32_t there = valid[n] >> (2 * (col % 16));
+          const auto seen = [&](int32_t at_v, uint32_t bit) {
+            return at_v <= part.hi[k] &&
+                   (p.window == 0 || at_v > part.hi[k] - p.window || at_v < p.sinks) && (bit & 1);
+          };
+          t.x = seen(v, there) ? t.x : -INFINITY;
+          t.y = seen(v + 1, there >> 2) ? t.y : -INFINITY;
+          t2 = pair(t.x, t.y);
         }
-        x[j] = exp2_approx(fmaf(t[j], part.a[k], ref));
+        top[k] = fmaxf(top[k], fmaxf(t.x, t.y));
+        x[h] = unpair(fma2(t2, a2[k], ref));
+        x[h].x = exp2_approx(x[h].x);
+        x[h].y = exp2_approx(x[h].y);
+        pr[4 * n + 2 * h + k] = pack_half2(x[h].x, x[h].y);
       }
-      part.top[k] = fmaxf(part.top[k], fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-      part.l[k] = fmaf((x[0] + x[1]) + (x[2] + x[3]), back, part.l[k]);
-      pr[4 * n + k] = pack_half2(x[0], x[1]);
-      pr[4 * n + 2 + k] = pack_half2(x[2], x[3]);
+      const float2 sum = unpair(add2(pair(x[0].x, x[0].y), pair(x[1].x, x[1].y)));
+      part.l[k] = fmaf(sum.x + sum.y, back, part.l[k]);
     }
   }
+  part.top[0] = top[0];
+  part.top[1] = top[1];
 }
 
 // A warp has 16 of a unit's rows: warps w and w + 4 have those of tensor memory
@@ -577,7 +639,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     const int row = warp_row + g + 8 * k;
     const float2 f = ctl.row[row];
     part.a[k] = f.x;
-    part.qsum[k] = f.y;
+    part.qsum[k] = pair(f.y, f.y);
     part.m[k] = -1e30f;
     l[k] = 0.0f;
     const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(first_row + row)));
@@ -603,16 +665,16 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
       const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
       all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu && v0 + kTok - 1 <= hi_first &&
             (p.window == 0 || v0 > hi_last - p.window || v0 + kTok - 1 < p.sinks);
-      const float4 ve = *reinterpret_cast<const float4*>(ctl.vexp[stage]);
-      vmax = fmaxf(fmaxf(ve.x, ve.y), fmaxf(ve.z, ve.w));
+      const float2* ve = ctl.vexp[stage];
+      vmax = fmaxf(fmaxf(ve[0].x, ve[1].x), fmaxf(ve[2].x, ve[3].x));
     }
     uint32_t pr[16];
     for (;;) {
       if (all) {
-        softmax_tile<true>(p, s_cols, ctl.kpar[stage], ctl.valid[stage], ctl.vexp[stage], v0, e,
+        softmax_tile<true>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
                            part, pr);
       } else {
-        softmax_tile<false>(p, s_cols, ctl.kpar[stage], ctl.valid[stage], ctl.vexp[stage], v0, e,
+        softmax_tile<false>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
                             part, pr);
       }
       bool grow = vmax - e > kExpSlack;
