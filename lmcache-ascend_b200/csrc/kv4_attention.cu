@@ -65,7 +65,7 @@ struct DecodeParams {
   int32_t stage_bytes;
   int32_t rows;    // query rows of a unit that may exist: max_query * group
   float* part;     // [2 * CTAs][heads][8 NT][D + 4]
-  int32_t* prefix; // [batch + 1]
+  int4* units;     // [groups * batch] where a unit's pieces are, for the join
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -131,6 +131,19 @@ __device__ __forceinline__ int32_t request_tiles(const AttnParams& p, const Requ
   if (r.n == 0) return 0;
   const KeyRange k = request_range(p, r);
   return k.count <= 0 ? 1 : (k.count + stage_tokens - 1) / stage_tokens;
+}
+
+// Of a unit that several CTAs work on, [first, last] with x < y, and in z the
+// first one's slot (its first piece, or its second where it had others before).
+__device__ __forceinline__ int4 unit_pieces(int64_t u0, int64_t u1, int64_t total, int64_t ctas) {
+  if (u1 <= u0) return make_int4(0, 0, 0, 0);
+  const auto cta_of = [&](int64_t x) {  // its tiles are [total c / ctas, total (c + 1) / ctas)
+    int64_t c = x * ctas / total;
+    while (total * (c + 1) / ctas <= x) ++c;
+    return static_cast<int>(c);
+  };
+  const int c0 = cta_of(u0), c1 = cta_of(u1 - 1);
+  return make_int4(c0, c1, 2 * c0 + (total * c0 / ctas >= u0 ? 0 : 1), 0);
 }
 
 // The CTAs that a line of `total` tiles is cut for.
@@ -410,11 +423,21 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
   }
 }
 
+// Warps that share a head add up in shared memory. Up to 128 values a row and 8
+// rows each has a place of its own there (32 KB), and all threads add them;
+// larger ones share a place, in turn.
+template <int D, int NT>
+__host__ __device__ constexpr bool own_places() {
+  return D * NT <= 128;
+}
+
 template <int D, int NT>
 __host__ __device__ constexpr size_t merge_bytes(int heads) {
   // one warp a head: nothing to merge
-  return kWarps / heads == 1 ? 0
-                             : (static_cast<size_t>(heads) * 8 * NT * (D + 1) + kWarps * 8 * NT) * 4;
+  return kWarps / heads == 1
+             ? 0
+             : ((own_places<D, NT>() ? kWarps : static_cast<size_t>(heads)) * 8 * NT * (D + 1) +
+                kWarps * 8 * NT) * 4;
 }
 
 // Where a query row's output, or this CTA's part of it, goes.
@@ -462,19 +485,20 @@ __device__ __forceinline__ void write_rows(const DecodeParams& p, const Request&
     }
 }
 
-// The same where several warps share a head: they add up in shared memory,
-// one after the other, then all write.
+// The same where several warps share a head.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request& rq, int group,
                                            int slot, const Running<D, NT>& st, float* smem) {
   constexpr int R = 8 * NT;
+  constexpr bool kOwn = own_places<D, NT>();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int heads = p.heads, turns = p.turns;
   const int head = warp % heads, turn = warp / heads;
   const bool working = turn < turns;
-  float* s_o = smem;                  // [heads][R][D]
-  float* s_l = s_o + heads * R * D;   // [heads][R]
-  float* s_m = s_l + heads * R;       // [kWarps][R], warps by turn
+  const int places = kOwn ? turns * heads : heads;
+  float* s_o = smem;                   // [places][R][D]
+  float* s_l = s_o + places * R * D;   // [places][R]
+  float* s_m = s_l + places * R;       // [turns][heads][R]
   if (working && g == 0) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -492,22 +516,24 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
       for (int w = 0; w < turns; ++w) m = fmaxf(m, s_m[(w * heads + head) * R + n * 8 + 2 * t + c]);
       f[n][c] = m == -INFINITY ? 0.0f : exp2_approx(st.m[n][c] - m);
     }
-  for (int w = 0; w < turns; ++w) {
-    if (w == turn) {
+  for (int w = 0; w < (kOwn ? 1 : turns); ++w) {
+    if (kOwn ? working : w == turn) {
+      const int place = kOwn ? turn * heads + head : head;
+      const bool add = !kOwn && w > 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int col = n * 8 + 2 * t + c;
           if (col >= p.rows) continue;
-          float* o = s_o + (head * R + col) * D + g * (D / 8);
+          float* o = s_o + (place * R + col) * D + g * (D / 8);
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             float2 v;
             v.x = fmaf(st.acc[i][n][c], unit, st.z[n][c]) * f[n][c];
             v.y = fmaf(st.acc[i][n][c + 2], unit16, st.z[n][c]) * f[n][c];
             float2* at = reinterpret_cast<float2*>(o + 2 * i);
-            if (w > 0) {
+            if (add) {
               const float2 old = *at;
               v.x += old.x;
               v.y += old.y;
@@ -516,7 +542,7 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
           }
           if (g == 0) {
             const float l = st.l[n][c] * f[n][c];
-            s_l[head * R + col] = w > 0 ? s_l[head * R + col] + l : l;
+            s_l[place * R + col] = add ? s_l[place * R + col] + l : l;
           }
         }
     }
@@ -528,8 +554,17 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
     const int kv_head = group * heads + h;
     const int tok = static_cast<int>(p.a.div_group.div(static_cast<uint32_t>(col)));
     if (tok >= rq.n || kv_head >= p.a.kv_heads) continue;
-    const float4 v = *reinterpret_cast<const float4*>(s_o + (h * R + col) * D + e);
-    const float l = s_l[h * R + col];
+    float4 v = *reinterpret_cast<const float4*>(s_o + (h * R + col) * D + e);
+    float l = s_l[h * R + col];
+    for (int w = 1; w < (kOwn ? turns : 1); ++w) {
+      const int place = w * heads + h;
+      const float4 u = *reinterpret_cast<const float4*>(s_o + (place * R + col) * D + e);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+      l += s_l[place * R + col];
+    }
     if (slot < 0) {
       const float inv = inverse_sum(l);
       const float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
@@ -771,11 +806,16 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   }
   if (threadIdx.x == 0) prefix[a.batch] = base;
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i <= a.batch; i += kThreads) p.prefix[i] = prefix[i];
-  }
   const int64_t total = static_cast<int64_t>(base) * p.groups;
   const int64_t n = active_ctas(total, gridDim.x);
+  // the last CTA has no more tiles than the others: it tells the join
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int i = threadIdx.x; i < a.batch * p.groups; i += kThreads) {
+      const int group = i / a.batch, b = i % a.batch;
+      const int64_t before = static_cast<int64_t>(group) * base;
+      p.units[i] = unit_pieces(before + prefix[b], before + prefix[b + 1], total, n);
+    }
+  }
   if (blockIdx.x >= n) return;
   Line line;
   line.prefix = prefix;
@@ -800,86 +840,83 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
 
 // Joins the pieces of every unit that more than one CTA worked on: one query
 // row for `parts` groups of D / 4 lanes, which share its pieces, always in the
-// same order.
-constexpr int kJoinThreads = 256;
+// same order. A lane has kPieces pieces on their way at once.
+constexpr int kJoinThreads = 512;
+constexpr int kPieces = 8;
+
+struct Merged {
+  float m, l;
+  float4 o;
+
+  __device__ __forceinline__ void add(float pm, float pl, const float4& v) {
+    const float nm = fmaxf(m, pm);
+    const float ref = nm == -INFINITY ? 0.0f : nm;
+    const float fa = exp2_approx(m - ref), fb = exp2_approx(pm - ref);
+    m = nm;
+    l = l * fa + pl * fb;
+    o.x = o.x * fa + v.x * fb;
+    o.y = o.y * fa + v.y * fb;
+    o.z = o.z * fa + v.z * fb;
+    o.w = o.w * fa + v.w * fb;
+  }
+};
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads)
-kv4_join_kernel(const __grid_constant__ DecodeParams p, const int num_ctas, const int parts) {
+kv4_join_kernel(const __grid_constant__ DecodeParams p, const int parts) {
   constexpr int kLanes = D / 4;
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads / kLanes];
   const AttnParams& a = p.a;
-  pdl_wait();
   const int who = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int part = who % parts;
-  const int row = blockIdx.x * (kJoinThreads / kLanes / parts) + who / parts;
+  const int row = blockIdx.x * (blockDim.x / kLanes / parts) + who / parts;
   const int b = blockIdx.y;
   const int kv_head = row / p.rows, col = row % p.rows;
   const int group = kv_head / p.heads, h = kv_head % p.heads;
   const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(col)));
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  pdl_wait();
+  Merged sum{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
   bool cut = false;
   Request rq{};
   if (kv_head < a.kv_heads) {
+    const int4 unit = p.units[group * a.batch + b];
     rq = load_request(a, b, false);
-    const int64_t per_group = p.prefix[a.batch];
-    const int64_t total = per_group * p.groups;
-    const int64_t u0 = group * per_group + p.prefix[b], u1 = group * per_group + p.prefix[b + 1];
-    if (tok < rq.n && u1 > u0) {
-      const int64_t n = active_ctas(total, num_ctas);
-      const auto cta_of = [&](int64_t x) {  // its tiles are [total c / n, total (c + 1) / n)
-        int64_t c = x * n / total;
-        while (total * (c + 1) / n <= x) ++c;
-        return static_cast<int>(c);
-      };
-      const int c0 = cta_of(u0), c1 = cta_of(u1 - 1);
-      cut = c0 != c1;  // else its CTA has written it
-      if (cut) {
-        // the unit is the first that a CTA works on, but in c0 where c0 had others before
-        const int slot0 = 2 * c0 + (total * c0 / n >= u0 ? 0 : 1);
-#pragma unroll 4
-        for (int c = c0 + part; c <= c1; c += parts) {
-          const float* src = part_row<D, NT>(p, c == c0 ? slot0 : 2 * c, h, col);
-          const float2 ml = *reinterpret_cast<const float2*>(src);
-          const float4 v = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
-          const float nm = fmaxf(m, ml.x);
-          const float ref = nm == -INFINITY ? 0.0f : nm;
-          const float fa = exp2_approx(m - ref), fb = exp2_approx(ml.x - ref);
-          m = nm;
-          l = l * fa + ml.y * fb;
-          o.x = o.x * fa + v.x * fb;
-          o.y = o.y * fa + v.y * fb;
-          o.z = o.z * fa + v.z * fb;
-          o.w = o.w * fa + v.w * fb;
+    cut = unit.x < unit.y && tok < rq.n;  // else its CTA has written it
+    if (cut) {
+      for (int c = unit.x + part; c <= unit.y; c += parts * kPieces) {
+        float2 ml[kPieces];
+        float4 v[kPieces];
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const int at = c + k * parts;
+          if (at <= unit.y) {
+            const float* src = part_row<D, NT>(p, at == unit.x ? unit.z : 2 * at, h, col);
+            ml[k] = *reinterpret_cast<const float2*>(src);
+            v[k] = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          if (c + k * parts <= unit.y) sum.add(ml[k].x, ml[k].y, v[k]);
         }
       }
     }
   }
   if (parts > 1) {
-    s_o[threadIdx.x] = o;
-    if (lane == 0) s_ml[who] = make_float2(m, l);
+    s_o[threadIdx.x] = sum.o;
+    if (lane == 0) s_ml[who] = make_float2(sum.m, sum.l);
     __syncthreads();
     if (part == 0) {
       for (int i = 1; i < parts; ++i) {
         const float2 ml = s_ml[who + i];
-        const float4 v = s_o[threadIdx.x + i * kLanes];
-        const float nm = fmaxf(m, ml.x);
-        const float ref = nm == -INFINITY ? 0.0f : nm;
-        const float fa = exp2_approx(m - ref), fb = exp2_approx(ml.x - ref);
-        m = nm;
-        l = l * fa + ml.y * fb;
-        o.x = o.x * fa + v.x * fb;
-        o.y = o.y * fa + v.y * fb;
-        o.z = o.z * fa + v.z * fb;
-        o.w = o.w * fa + v.w * fb;
+        sum.add(ml.x, ml.y, s_o[threadIdx.x + i * kLanes]);
       }
     }
   }
   if (!cut || part != 0) return;
-  const float inv = inverse_sum(l);
-  const float x[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const float inv = inverse_sum(sum.l);
+  const float x[4] = {sum.o.x * inv, sum.o.y * inv, sum.o.z * inv, sum.o.w * inv};
   store_out<T, 4>(static_cast<T*>(a.out) + (rq.row0 + static_cast<int64_t>(tok)) * a.out_stride +
                       static_cast<int64_t>(kv_head * a.group + col - tok * a.group) * D + lane * 4,
                   a.out_vec != 0, x);
@@ -895,7 +932,7 @@ struct Plan {
   int heads, turns, groups;
   int stage_tokens, tok_stride, stage_bytes, stages;
   int ctas;
-  int64_t part_bytes, prefix_bytes;
+  int64_t part_bytes, unit_bytes;
 };
 
 Plan make_plan(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_heads, int64_t group,
@@ -913,7 +950,9 @@ Plan make_plan(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_hea
   pl.stage_bytes = 2 * pl.stage_tokens * pl.tok_stride;
   const int per_sm = head_size * pl.nt <= 128 ? 2 : 1;
   const int64_t merge =
-      pl.turns == 1 ? 0 : (pl.heads * 8 * pl.nt * (head_size + 1) + kWarps * 8 * pl.nt) * 4;
+      pl.turns == 1 ? 0
+                    : ((head_size * pl.nt <= 128 ? kWarps : pl.heads) * 8 * pl.nt * (head_size + 1) +
+                       kWarps * 8 * pl.nt) * 4;
   const int64_t room = 220 * 1024 / per_sm - merge - (batch + 1) * 4 - 1024;
   pl.stages = static_cast<int>(room / pl.stage_bytes);
   if (pl.stages > kMaxStages) pl.stages = kMaxStages;
@@ -924,7 +963,7 @@ Plan make_plan(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_hea
   const int64_t most = static_cast<int64_t>(current_sm_count()) * per_sm;
   if (tiles > most) tiles = most;
   pl.ctas = static_cast<int>(tiles < 1 ? 1 : tiles);
-  pl.prefix_bytes = (batch + 1 + 63) / 64 * 256;
+  pl.unit_bytes = batch * pl.groups * 16;
   pl.part_bytes = int64_t(2) * pl.ctas * pl.heads * pl.nt * 8 * (head_size + 4) * 4;
   return pl;
 }
@@ -940,24 +979,24 @@ cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t stream) {
   kv4_decode_kernel<T, D, NT, ST><<<pl.ctas, kThreads, smem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  // Few long requests: the pieces of a row are shared by several lane groups.
+  // Few long requests: the pieces of a row are shared by several lane groups, so
+  // that each has no more than it takes at once.
   int parts = 1;
-  const int lane_groups = kJoinThreads / (D / 4);
-  while (parts < lane_groups && static_cast<int64_t>(pl.ctas) > 4 * parts * p.a.batch * p.groups) {
-    parts *= 2;
-  }
-  const int per_block = lane_groups / parts;
+  const int64_t pieces = pl.ctas / (static_cast<int64_t>(p.a.batch) * p.groups);
+  while (parts < kJoinThreads / (D / 4) && pieces > parts * kPieces) parts *= 2;
+  const int threads = parts * (D / 4) > 256 ? kJoinThreads : 256;
+  const int per_block = threads / (D / 4) / parts;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.a.kv_heads * p.rows + per_block - 1) / per_block),
                      static_cast<unsigned>(p.a.batch));
-  cfg.blockDim = dim3(kJoinThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D, NT>, p, pl.ctas, parts);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D, NT>, p, parts);
 }
 
 template <typename T>
@@ -1024,7 +1063,7 @@ int lmcb_kv4_attention_workspace(int64_t batch, int64_t maxQueryLen, int64_t max
   if (kv4::is_decode(maxQueryLen, group)) {
     const kv4::Plan pl = kv4::make_plan(batch, maxQueryLen, maxSeqLen, numKvHeads, group, headSize,
                                         window, sinks);
-    *bytesOut = static_cast<size_t>(pl.part_bytes + pl.prefix_bytes);
+    *bytesOut = static_cast<size_t>(pl.part_bytes + pl.unit_bytes);
   } else {
     *bytesOut = kv4::rows_workspace(batch, maxQueryLen, maxSeqLen, numKvHeads, group, headSize,
                                     window, sinks);
@@ -1116,7 +1155,7 @@ int lmcb_kv4_attention(const void* query, int type, int64_t queryTokenStride, in
     p.stage_bytes = pl.stage_bytes;
     p.rows = static_cast<int32_t>(maxQueryLen * a.group);
     p.part = static_cast<float*>(workspace);
-    p.prefix = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + pl.part_bytes);
+    p.units = reinterpret_cast<int4*>(static_cast<char*>(workspace) + pl.part_bytes);
     err = type == LMCB_DTYPE_BF16 ? kv4::launch_size<__nv_bfloat16>(p, pl, headSize, s)
                                   : kv4::launch_size<__half>(p, pl, headSize, s);
   } else {

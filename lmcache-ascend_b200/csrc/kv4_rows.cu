@@ -12,9 +12,12 @@
 // 16 c, c 2^-24; Q's odd elements carry the 1/16), so a logit is an fp32 sum of
 // exact products. V is made fp16 on the way, v 2^-e with 2^e above the largest
 // of its 16 tokens; P takes the 2^e, relative to the row's own E, so neither
-// loses small caches nor overflows. The rounding of v and of p are 2^-12 each
-// of their own size: dequantising V costs 128 rows nothing, where taking sv
-// into P, as the decode kernel does, would cost every element of S.
+// loses small caches nor overflows. Both are rounded to fp16 once; for bf16
+// results that is an eighth of their own rounding. fp16 results are rounded no
+// more coarsely than V and P: they take P as two fp16 numbers, p and what its
+// rounding left, in a second product, which leaves V's rounding alone (error
+// against 64 bits 2.9e-4 of the result's size, 2.1e-4 is the result's own, and
+// 3.4e-4 with one number).
 //
 // A CTA has two such units (one for D = 256), 256 query rows, which share the
 // tiles. Per tile the tensor core needs 1024 cycles for them, the exponentials
@@ -31,6 +34,7 @@
 // O stays in tensor memory; it is rescaled only when a row's reference grows by
 // more than 2^8, which P's range leaves room for.
 #include <climits>
+#include <type_traits>
 
 #include "kv4_attention.cuh"
 #include "kv4_plan.h"
@@ -155,8 +159,25 @@ __device__ __forceinline__ void tmem_store_rows_f32(uint32_t addr, const uint32_
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_wait_load() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// The registers of a load are there after its wait: they pass through it.
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_store() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -494,47 +515,68 @@ __device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t stage,
   }
 }
 
-// Q K^T runs a tile ahead of P V: softmax finds the next S when it is done with
-// one.
-template <int D>
-__device__ __forceinline__ bool issue(int32_t tiles, int units, uint32_t smem, Control& ctl) {
+// Q K^T runs ahead of P V: softmax finds the next S when it is done with one.
+// Only products into the same accumulator keep their order by themselves. So
+// Q K^T of tile j waits until the P V of tile j - 2, whose P lay in the same S,
+// has ended; with two units, each one's P V is waited for while the other's
+// runs.
+template <int D, bool kTwo>
+struct Issuer {
   using L = Layout<D>;
-  const uint32_t tmem = ctl.tmem, stages = smem + L::kUnits * L::kQ;
-  int stage = 0, qk_stage = 0;
-  uint32_t qk_phase = 0;
-  for (int32_t i = -1; i < tiles; ++i) {
-    if (i + 1 < tiles) {
-      if (!mbar_wait(&ctl.full[qk_stage], qk_phase)) return false;
-      fence_after();
-      if (elect_one()) {
-        const int buf = (i + 1) & 1;
-        for (int u = 0; u < units; ++u) {
-          // into the S whose P the product of tile i - 1 reads: products run in order
-          issue_qk<D>(tmem + u * L::kUnit + buf * kTok, smem + u * L::kQ,
-                      stages + qk_stage * L::kStage);
-          commit(&ctl.sready[u][buf]);
-        }
-      }
-      __syncwarp();
-      if (++qk_stage == L::kStages) qk_stage = 0, qk_phase ^= 1;
+  uint32_t tmem, rows, stages;
+  int units;
+  Control& ctl;
+
+  __device__ __forceinline__ bool qk(int u, int32_t j) const {
+    const int stage = j % L::kStages, buf = j & 1;
+    if (!mbar_wait(&ctl.full[stage], (j / L::kStages) & 1)) return false;
+    if (j >= 2 && !mbar_wait(&ctl.pvdone[u], j & 1)) return false;
+    fence_after();
+    if (elect_one()) {
+      issue_qk<D>(tmem + u * L::kUnit + buf * kTok, rows + u * L::kQ, stages + stage * L::kStage);
+      commit(&ctl.sready[u][buf]);
     }
-    if (i < 0) continue;
-    const int buf = i & 1;
-    for (int u = 0; u < units; ++u) {
-      if (!mbar_wait(&ctl.pready[u][buf], (i >> 1) & 1)) return false;
-      fence_after();
-      if (elect_one()) {
-        const uint32_t unit = tmem + u * L::kUnit;
-        issue_pv<D>(unit + L::kO, unit + buf * kTok, stages + stage * L::kStage, i > 0);
-        commit(&ctl.pvdone[u]);
-        if (u == units - 1) commit(&ctl.free[stage]);
-      }
-      __syncwarp();
-    }
-    if (++stage == L::kStages) stage = 0;
+    __syncwarp();
+    return true;
   }
-  return true;
-}
+
+  __device__ __forceinline__ bool pv(int u, int32_t j) const {
+    const int stage = j % L::kStages, buf = j & 1;
+    if (!mbar_wait(&ctl.pready[u][buf], (j >> 1) & 1)) return false;
+    fence_after();
+    if (elect_one()) {
+      const uint32_t unit = tmem + u * L::kUnit, p = unit + buf * kTok;
+      issue_pv<D>(unit + L::kO, p, stages + stage * L::kStage, j > 0);
+      if constexpr (kTwo) {
+        issue_pv<D>(unit + L::kO, p + kTok / 2, stages + stage * L::kStage, true);
+      }
+      commit(&ctl.pvdone[u]);
+      if (u == units - 1) commit(&ctl.free[stage]);
+    }
+    __syncwarp();
+    return true;
+  }
+
+  __device__ __forceinline__ bool run(int32_t tiles) const {
+    if (tiles == 0) return true;
+    if (!qk(0, 0)) return false;
+    if (units == 1) {
+      for (int32_t j = 0; j < tiles; ++j) {
+        if (j + 1 < tiles && !qk(0, j + 1)) return false;
+        if (!pv(0, j)) return false;
+      }
+      return true;
+    }
+    if (!qk(1, 0) || (tiles > 1 && !qk(0, 1))) return false;
+    for (int32_t j = 0; j < tiles; ++j) {
+      if (!pv(0, j)) return false;
+      if (j + 1 < tiles && !qk(1, j + 1)) return false;
+      if (!pv(1, j)) return false;
+      if (j + 2 < tiles && !qk(0, j + 2)) return false;
+    }
+    return true;
+  }
+};
 
 // ---------------------------------------------------------------------------
 // The warps that have the query rows
@@ -553,11 +595,11 @@ struct Part {
 
 // S into P and the rows' largest t and sums. `ve` are the exponents of V's 16
 // tokens each, `e` the warp's.
-template <bool kAll>
+template <bool kAll, bool kTwo>
 __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_cols,
                                              const ulonglong2* kpar, const uint32_t* valid,
                                              const float2* vexp, int32_t v0, float e, Part& part,
-                                             uint32_t (&pr)[16]) {
+                                             uint32_t (&pr)[16], uint32_t (&rest)[16]) {
   const int t4 = threadIdx.x % 4;
   uint32_t s[32];
   tmem_load_rows(s, s_cols);
@@ -571,7 +613,7 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
     top[k] = -INFINITY;
     part.l[k] = 0.0f;
   }
-  tmem_wait_load();
+  tmem_wait_load(s);
 #pragma unroll
   for (int n = 0; n < 4; ++n) {  // 16 tokens: one exponent of V
     const uint64_t ve = *reinterpret_cast<const uint64_t*>(&vexp[n]);
@@ -602,7 +644,11 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
         x[h] = unpair(fma2(t2, a2[k], ref));
         x[h].x = exp2_approx(x[h].x);
         x[h].y = exp2_approx(x[h].y);
-        pr[4 * n + 2 * h + k] = pack_half2(x[h].x, x[h].y);
+        const uint32_t r = pack_half2(x[h].x, x[h].y);
+        pr[4 * n + 2 * h + k] = r;
+        if constexpr (kTwo) {
+          rest[4 * n + 2 * h + k] = pack_half2(x[h].x - half_lo(r), x[h].y - half_hi(r));
+        }
       }
       const float2 sum = unpair(add2(pair(x[0].x, x[0].y), pair(x[1].x, x[1].y)));
       part.l[k] = fmaf(sum.x + sum.y, back, part.l[k]);
@@ -618,7 +664,7 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
 // there; only a tile that outgrows them by the slack (the first one, and few
 // after it) is taken again, with new ones. So nothing waits for a tile's
 // maximum, and a thread never holds more than the tile's S.
-template <int D>
+template <int D, bool kTwo>
 __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& range, int32_t t0,
                                        int32_t tiles, int32_t pos_first, int32_t pos_last,
                                        const Request& rq, int first_row, Control& ctl) {
@@ -668,14 +714,14 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
       const float2* ve = ctl.vexp[stage];
       vmax = fmaxf(fmaxf(ve[0].x, ve[1].x), fmaxf(ve[2].x, ve[3].x));
     }
-    uint32_t pr[16];
+    uint32_t pr[16], rest[16];
     for (;;) {
       if (all) {
-        softmax_tile<true>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
-                           part, pr);
+        softmax_tile<true, kTwo>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
+                           part, pr, rest);
       } else {
-        softmax_tile<false>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
-                            part, pr);
+        softmax_tile<false, kTwo>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
+                            part, pr, rest);
       }
       bool grow = vmax - e > kExpSlack;
 #pragma unroll
@@ -705,7 +751,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
         for (int c = 0; c < D; c += 32) {
           uint32_t o[16];
           tmem_load_rows(o, mine + L::kO + c);
-          tmem_wait_load();
+          tmem_wait_load(o);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha[j / 2 % 2]);
@@ -715,6 +761,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
       }
     }
     tmem_store_rows(s_cols, pr);
+    if constexpr (kTwo) tmem_store_rows(s_cols + kTok / 2, rest);
 #pragma unroll
     for (int k = 0; k < 2; ++k) l[k] += part.l[k];
     tmem_wait_store();
@@ -758,7 +805,7 @@ __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq
     __syncwarp();
     if (any) {  // uniform: the whole CTA had tiles
       tmem_load32(o, mine + L::kO + c);
-      tmem_wait_load();
+      tmem_wait_load(o);
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) o[j] = 0;
@@ -800,6 +847,8 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   pdl_launch_dependents();
   const Request rq =
       load_request(a, b, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
+  // fp16 results show the rounding of P: they take P in two parts
+  constexpr bool kTwo = std::is_same<T, __half>::value;
   constexpr int kCtaRows = kRows * L::kUnits;
   const int64_t rows = static_cast<int64_t>(rq.n) * a.group;
   if (static_cast<int64_t>(tile) * kCtaRows >= rows) return;
@@ -856,13 +905,16 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   bool ok = true;
   if (warp >= L::kIssue) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    if (warp == L::kIssue) ok = issue<D>(t1 - t0, units, smem_u32(smem), ctl);
+    if (warp == L::kIssue) {
+      const uint32_t q = smem_u32(smem);
+      ok = Issuer<D, kTwo>{ctl.tmem, q, q + L::kUnits * L::kQ, units, ctl}.run(t1 - t0);
+    }
   } else if (warp >= L::kBring) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     ok = bring<D>(a, range, b, kv_head, t0, t1 - t0, smem + L::kUnits * L::kQ, ctl);
   } else if (warp < 8 * units) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
-    ok = attend<D>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, ctl);
+    ok = attend<D, kTwo>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, ctl);
     asm volatile("bar.sync %0, 256;" ::"r"(1 + unit) : "memory");  // the unit's rows are done
     float* part = nullptr;
     if (p.splits > 1) {

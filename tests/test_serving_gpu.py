@@ -592,6 +592,20 @@ def test_attention_window_and_sinks(window, sinks, qlens):
     b.check(b.run(window, sinks), window, sinks, rows=[0, 1, 5, 31, 32, 64, -1])
 
 
+@pytest.mark.parametrize("dtype,window", [(torch.bfloat16, 0), (torch.float16, 0),
+                                          (torch.float16, 1500)])
+@pytest.mark.parametrize("d,hkv,group", [(128, 2, 8), (64, 1, 16), (256, 1, 4)])
+def test_attention_long_suffix(dtype, window, d, hkv, group):
+    """Hundreds of query rows over thousands of keys: every ring and buffer goes
+    round many times, and every run gives the same bits."""
+    b = Batch([5000, 700, 2500], [260, 70, 1], hkv, group, d, 16, dtype, seed=d)
+    out = b.run(window, 4 if window else 0)
+    b.check(out, window, 4 if window else 0, rows=[0, 17, 128, 255, -1])
+    for _ in range(10):
+        assert torch.equal(b.run(window, 4 if window else 0), out)
+    assert c_ops.device_status(0) == 0
+
+
 def test_attention_queries_before_the_cache():
     """More queries than tokens: the first ones stand before position 0 and see
     nothing, so their rows are zeros."""
