@@ -154,38 +154,44 @@ __device__ __forceinline__ void row_range(const Eight<T>& x, bool active, float&
   }
 }
 
-// One word of codes clamp(rne((x - z) / s), 0, 15) in 64 bits.
-__device__ __noinline__ uint32_t exact_word(const float (&v)[8], float z, float s) {
-  uint32_t word = 0;
-  for (int i = 0; i < 8; ++i) {
-    const double q = (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
-    word |= static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0)) << (4 * i);
-  }
-  return word;
-}
-
-// The same in fp32: q is off by less than 2^-17 (a rounded difference, an
-// approximate reciprocal of 1 ulp and a rounded product, each 2^-23 of at most
-// 16 + 2^-6 before the clamp), so only a q that close to a border between two
-// codes needs more. Adding 1.5 2^23 rounds q to an integer, ties to even, in
-// the sum's low bits; a multiply-add by 16^i puts it in its place, and what the
-// eight exponent fields add up to is one constant.
+// One word of codes clamp(rne((x - z) / s), 0, 15).
+//
+// In fp32, y = x / (15 s) - z / (15 s) with an approximate reciprocal, clamped to
+// [0, 1] by the multiply-add itself, is off by less than (|x| + |z|) / (15 s)
+// 2^-22 <= (2 |z| / s / 15 + 1) 2^-22, so 15 y by (|z| / s + 8) 2^-21. Adding
+// 1.5 2^23 rounds 15 y to an integer, ties to even, in the sum's low bits; a
+// multiply-add by 16^i puts it in its place, and what the eight exponent fields
+// add up to is one constant. Only an element that lies that close to the border
+// between two codes is taken again, in 64 bits: three in a hundred thousand.
 __device__ __forceinline__ uint32_t word_of(const float (&v)[8], float z, float s) {
   constexpr float kMagic = 12582912.0f;
   constexpr uint32_t kBias = 0x4B400000u * 0x11111111u;
   float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.0f * s));
+  const float shift = -z * inv;
+  const float sure = 0.5f - fmaf(fabsf(shift), 15.0f, 8.0f) * 4.7683716e-7f;
   uint32_t word = 0;
   float off = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = fminf(fmaxf((v[i] - z) * inv, 0.0f), 15.0f);
-    const float r = q + kMagic;
-    off = fmaxf(off, fabsf(q - (r - kMagic)));
+    const float y = __saturatef(fmaf(v[i], inv, shift));
+    const float r = fmaf(y, 15.0f, kMagic);
+    off = fmaxf(off, fabsf(fmaf(y, 15.0f, kMagic - r)));
     word += __float_as_uint(r) << (4 * i);
   }
   word -= kBias;
-  if (off > 0.5f - 1.0f / 65536.0f) word = exact_word(v, z, s);
+  if (off >= sure) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = __saturatef(fmaf(v[i], inv, shift));
+      if (fabsf(fmaf(y, 15.0f, kMagic - fmaf(y, 15.0f, kMagic))) >= sure) {
+        const double q =
+            (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
+        const uint32_t code = static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
+        word = (word & ~(15u << (4 * i))) | (code << (4 * i));
+      }
+    }
+  }
   return word;
 }
 

@@ -25,7 +25,7 @@
 namespace lmcb {
 namespace {
 
-constexpr int kBatchThreads = 512;
+constexpr int kBatchThreads = 1024;  // 256 for a batch that they cover
 constexpr int kBatchMaxRequests = 16384;  // 12 bytes of shared memory each
 constexpr int kTokensPerThread = 4;
 
@@ -43,6 +43,7 @@ struct BatchParams {
   int32_t num_tokens;
   void* slots;
   void* positions;
+  int aligned;  // slots and positions start on 16 bytes
   int32_t* query_start;
   int32_t* seq_lens;
   int32_t* blocks_used;
@@ -84,19 +85,38 @@ __device__ __forceinline__ int last_le(const int32_t* a, int n, int32_t key) {
   return lo;
 }
 
+// Sums that stop at INT_MAX: what lies behind it is behind every table and
+// every token too.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  return min(a + b, static_cast<uint32_t>(INT_MAX));
+}
+
+// Inclusive sums over a warp.
+__device__ __forceinline__ void warp_sums(uint32_t& a, uint32_t& b, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, a, o);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a = add_sat(a, x);
+      b = add_sat(b, y);
+    }
+  }
+}
+
 template <typename SlotT>
 __global__ void __launch_bounds__(kBatchThreads) build_slot_mapping_kernel(const BatchParams p) {
   extern __shared__ int32_t batch_smem[];
   const int B = p.num_requests;
-  int32_t* s_start = batch_smem;      // [B] first token of the request
-  int32_t* s_first = s_start + B;     // [B] first free-list entry of the request
-  int32_t* s_ctx = s_first + B;       // [B] tokens in the cache
-  __shared__ int64_t s_warp[2][kBatchThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* s_start = batch_smem;  // [B] first token of the request
+  int32_t* s_first = s_start + B; // [B] first free-list entry of the request
+  int32_t* s_ctx = s_first + B;   // [B] tokens in the cache
+  __shared__ uint32_t s_warp[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
 
-  // Prefix sums, kBatchThreads requests at a time, in 64 bits.
-  int64_t base_tok = 0, base_page = 0;
-  for (int b0 = 0; b0 < B; b0 += kBatchThreads) {
+  // Prefix sums, a request a thread and round.
+  uint32_t base_tok = 0, base_page = 0;
+  for (int b0 = 0; b0 < B; b0 += threads) {
     const int b = b0 + tid;
     int32_t ctx = 0, fresh = 0, need = 0;
     if (b < B) {
@@ -105,61 +125,60 @@ __global__ void __launch_bounds__(kBatchThreads) build_slot_mapping_kernel(const
       need = pages_of(static_cast<int64_t>(ctx) + fresh, p.div_block, p.table_cols) -
              pages_of(ctx, p.div_block, p.table_cols);
     }
-    int64_t tok = fresh, page = need;  // inclusive sums of the warp
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t a = __shfl_up_sync(0xffffffffu, tok, o);
-      const int64_t c = __shfl_up_sync(0xffffffffu, page, o);
-      if (lane >= o) {
-        tok += a;
-        page += c;
-      }
-    }
+    uint32_t tok = fresh, page = need;
+    warp_sums(tok, page, lane);
     if (lane == 31) {
       s_warp[0][warp] = tok;
       s_warp[1][warp] = page;
     }
     __syncthreads();
-    int64_t before_tok = base_tok, before_page = base_page;
-    for (int w = 0; w < kBatchThreads / 32; ++w) {
-      if (w < warp) {
-        before_tok += s_warp[0][w];
-        before_page += s_warp[1][w];
-      }
-      base_tok += s_warp[0][w];
-      base_page += s_warp[1][w];
+    if (warp == 0) {
+      uint32_t t = lane < threads / 32 ? s_warp[0][lane] : 0;
+      uint32_t g = lane < threads / 32 ? s_warp[1][lane] : 0;
+      warp_sums(t, g, lane);
+      s_warp[0][lane] = t;
+      s_warp[1][lane] = g;
     }
+    __syncthreads();
+    const uint32_t before_tok = warp > 0 ? add_sat(base_tok, s_warp[0][warp - 1]) : base_tok;
+    const uint32_t before_page = warp > 0 ? add_sat(base_page, s_warp[1][warp - 1]) : base_page;
     if (b < B) {
+      // this thread's own come off again, but for sums that have stopped
+      const uint32_t tok_sum = add_sat(before_tok, tok), page_sum = add_sat(before_page, page);
+      const uint32_t st = tok_sum == INT_MAX ? tok_sum : tok_sum - fresh;
       s_ctx[b] = ctx;
-      const int64_t st = before_tok + tok - fresh;
-      s_start[b] = static_cast<int32_t>(st < p.num_tokens ? st : p.num_tokens);
-      s_first[b] = clamp31(before_page + page - need);
+      s_start[b] = static_cast<int32_t>(min(st, static_cast<uint32_t>(p.num_tokens)));
+      s_first[b] = static_cast<int32_t>(page_sum == INT_MAX ? page_sum : page_sum - need);
       if (blockIdx.x == 0) {
         p.query_start[b] = s_start[b];
         p.seq_lens[b] = clamp31(static_cast<int64_t>(ctx) + fresh);
       }
     }
+    base_tok = add_sat(base_tok, s_warp[0][31]);
+    base_page = add_sat(base_page, s_warp[1][31]);
     __syncthreads();  // s_warp is rewritten by the next round
   }
   const int32_t total_tok =
-      static_cast<int32_t>(base_tok < p.num_tokens ? base_tok : p.num_tokens);
-  const int32_t total_page = clamp31(base_page);
+      static_cast<int32_t>(min(base_tok, static_cast<uint32_t>(p.num_tokens)));
+  const int32_t total_page = static_cast<int32_t>(base_page);
   if (blockIdx.x == 0 && tid == 0) {
     p.query_start[B] = total_tok;
     p.blocks_used[0] = total_page;
-    if (base_tok > p.num_tokens) raise_flag(p.status, LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE);
+    if (base_tok > static_cast<uint32_t>(p.num_tokens)) {
+      raise_flag(p.status, LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE);
+    }
     if (total_page > p.num_free) raise_flag(p.status, LMCB_DEVICE_FLAG_PAGES_EXHAUSTED);
   }
 
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBatchThreads;
-  const int64_t me = static_cast<int64_t>(blockIdx.x) * kBatchThreads + tid;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * threads;
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * threads + tid;
 
   // New table entries, one a thread.
   for (int64_t e = me; e < total_page; e += stride) {
     const int r = last_le(s_first, B, static_cast<int32_t>(e));
     const int32_t col = pages_of(s_ctx[r], p.div_block, p.table_cols) +
                         static_cast<int32_t>(e - s_first[r]);
-    // Inside the row by construction; the test also covers sums beyond 2^31.
+    // Inside the row by construction; the test also covers sums that stopped.
     if (col < p.table_cols) {
       p.table[r * p.table_stride + col] = e < p.num_free ? p.free_blocks[e] : -1;
     }
@@ -168,51 +187,66 @@ __global__ void __launch_bounds__(kBatchThreads) build_slot_mapping_kernel(const
   // Slots and positions, kTokensPerThread consecutive tokens a thread.
   SlotT* slots = static_cast<SlotT*>(p.slots);
   SlotT* positions = static_cast<SlotT*>(p.positions);
+  const int64_t row_tokens = static_cast<int64_t>(p.table_cols) * p.div_block.d;
   for (int64_t t0 = me * kTokensPerThread; t0 < p.num_tokens; t0 += stride * kTokensPerThread) {
+    alignas(16) SlotT slot[kTokensPerThread], position[kTokensPerThread];
     int r = 0;
-    int32_t r_end = 0;  // first token behind request r
-    int32_t cached_blk = -1, cached_page = -1;
+    int32_t r_start = 0, r_end = 0, r_ctx = 0, r_has = 0;  // of request r, tokens [start, end)
+    int32_t blk = -1, page = -1;
 #pragma unroll
     for (int k = 0; k < kTokensPerThread; ++k) {
       const int32_t t = static_cast<int32_t>(t0) + k;
-      if (t0 + k >= p.num_tokens) break;
-      if (t >= total_tok) {
-        slots[t] = -1;
-        positions[t] = 0;
+      slot[k] = -1;
+      position[k] = 0;
+      if (t >= total_tok) continue;
+      if (t >= r_end) {
+        r = last_le(s_start, B, t);
+        r_start = s_start[r];
+        r_end = r + 1 < B ? s_start[r + 1] : total_tok;
+        r_ctx = s_ctx[r];
+        r_has = pages_of(r_ctx, p.div_block, p.table_cols);
+        blk = -1;
+      }
+      const int64_t pos = static_cast<int64_t>(r_ctx) + (t - r_start);
+      position[k] = static_cast<SlotT>(pos);
+      if (pos >= row_tokens) {
+        raise_flag(p.status, LMCB_DEVICE_FLAG_PAGES_EXHAUSTED);  // beyond the table's row
         continue;
       }
-      if (k == 0 || t >= r_end) {
-        r = last_le(s_start, B, t);
-        r_end = r + 1 < B ? s_start[r + 1] : total_tok;
-        cached_blk = -1;
-      }
-      const int64_t pos = static_cast<int64_t>(s_ctx[r]) + (t - s_start[r]);
-      int64_t slot = -1;
-      if (pos < static_cast<int64_t>(p.table_cols) * p.div_block.d) {
-        const int32_t blk = static_cast<int32_t>(p.div_block.div(static_cast<uint32_t>(pos)));
-        if (blk != cached_blk) {
-          cached_blk = blk;
-          const int32_t has = pages_of(s_ctx[r], p.div_block, p.table_cols);
-          if (blk < has) {
-            cached_page = p.table[r * p.table_stride + blk];
-          } else {
-            const int64_t f = static_cast<int64_t>(s_first[r]) + (blk - has);
-            cached_page = f < p.num_free ? p.free_blocks[f] : -1;
-          }
+      const int32_t b = static_cast<int32_t>(p.div_block.div(static_cast<uint32_t>(pos)));
+      if (b != blk) {
+        blk = b;
+        if (blk < r_has) {
+          page = p.table[r * p.table_stride + blk];
+        } else {
+          const int64_t f = static_cast<int64_t>(s_first[r]) + (blk - r_has);
+          page = f < p.num_free ? p.free_blocks[f] : -1;
         }
-        if (cached_page >= 0) {
-          slot = static_cast<int64_t>(cached_page) * p.div_block.d +
-                 (pos - static_cast<int64_t>(blk) * p.div_block.d);
-          if (sizeof(SlotT) == 4 && slot > INT_MAX) {
-            raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
-            slot = -1;
-          }
-        }
-      } else {
-        raise_flag(p.status, LMCB_DEVICE_FLAG_PAGES_EXHAUSTED);  // beyond the table's row
       }
-      slots[t] = static_cast<SlotT>(slot);
-      positions[t] = static_cast<SlotT>(pos);
+      if (page < 0) continue;
+      const int64_t at = static_cast<int64_t>(page) * p.div_block.d +
+                         (pos - static_cast<int64_t>(blk) * p.div_block.d);
+      if (sizeof(SlotT) == 4 && at > INT_MAX) {
+        raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
+        continue;
+      }
+      slot[k] = static_cast<SlotT>(at);
+    }
+    if (p.aligned && t0 + kTokensPerThread <= p.num_tokens) {
+      constexpr int kVecs = sizeof(slot) / 16;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        reinterpret_cast<uint4*>(slots + t0)[v] = reinterpret_cast<const uint4*>(slot)[v];
+        reinterpret_cast<uint4*>(positions + t0)[v] = reinterpret_cast<const uint4*>(position)[v];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kTokensPerThread; ++k) {
+        if (t0 + k < p.num_tokens) {
+          slots[t0 + k] = slot[k];
+          positions[t0 + k] = position[k];
+        }
+      }
     }
   }
 }
@@ -265,24 +299,28 @@ int lmcb_build_slot_mapping(const void* contextLens, const void* queryLens, int 
   p.num_tokens = static_cast<int32_t>(numTokens);
   p.slots = slotMapping;
   p.positions = positions;
+  p.aligned = reinterpret_cast<uintptr_t>(slotMapping) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(positions) % 16 == 0;
   p.query_start = queryStart;
   p.seq_lens = seqLens;
   p.blocks_used = blocksUsed;
   p.status = lmcb::device_status_ptr();
   if (p.status == nullptr) return LMCB_ERR_CUDA;
-  const int64_t per_cta = int64_t(lmcb::kBatchThreads) * lmcb::kTokensPerThread;
-  const int64_t want = (numTokens + per_cta - 1) / per_cta;
-  const int64_t most = static_cast<int64_t>(lmcb::current_sm_count()) * 2;
+  const int64_t groups =
+      (numTokens + lmcb::kTokensPerThread - 1) / lmcb::kTokensPerThread;
+  const int threads = groups <= 256 && numRequests <= 256 ? 256 : lmcb::kBatchThreads;
+  const int64_t want = (groups + threads - 1) / threads;
+  const int64_t most = lmcb::current_sm_count();
   const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
   const size_t smem = static_cast<size_t>(numRequests) * 12;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   constexpr size_t kCap = size_t(lmcb::kBatchMaxRequests) * 12;
   if (slotType == LMCB_DTYPE_INT64) {
     LMCB_CUDA_TRY((lmcb::ensure_smem_limit<lmcb::build_slot_mapping_kernel<int64_t>>(smem, kCap)));
-    lmcb::build_slot_mapping_kernel<int64_t><<<grid, lmcb::kBatchThreads, smem, s>>>(p);
+    lmcb::build_slot_mapping_kernel<int64_t><<<grid, threads, smem, s>>>(p);
   } else {
     LMCB_CUDA_TRY((lmcb::ensure_smem_limit<lmcb::build_slot_mapping_kernel<int32_t>>(smem, kCap)));
-    lmcb::build_slot_mapping_kernel<int32_t><<<grid, lmcb::kBatchThreads, smem, s>>>(p);
+    lmcb::build_slot_mapping_kernel<int32_t><<<grid, threads, smem, s>>>(p);
   }
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return lmcb::cuda_fail(err, who.c_str());

@@ -470,7 +470,7 @@ constexpr int kQkRowsInFlight = 2;
 // cos/sin values a lane needs are the same for every head, so it loads them
 // once for the run.
 template <typename T, bool kNeox, int kLanes>
-__global__ void __launch_bounds__(kQkThreads)
+__global__ void __launch_bounds__(kQkThreads, 3)
 qk_norm_rope_vec_kernel(const QkNormParams p, const uint32_t num_items, const FastDiv div_runs,
                         const int heads_per_run) {
   constexpr int E = 16 / sizeof(T);
