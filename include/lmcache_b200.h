@@ -394,7 +394,8 @@ LMCB_API int lmcb_rotary_embedding_k_fused(const void* oldPositions, const void*
  * A free list that runs out gives table entries and slots of -1 and sets
  * LMCB_DEVICE_FLAG_PAGES_EXHAUSTED, as tokens behind a table row's end do.
  * Negative lengths count as 0, and tokens that do not fit numTokens are left
- * out (queryStart stops at numTokens); both set
+ * out with the pages that would start with them (queryStart stops at
+ * numTokens); both set
  * LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE. At most 16384 requests
  * (LMCB_ERR_CAPACITY). No output may overlap an input or another output. */
 LMCB_API int lmcb_build_slot_mapping(const void* contextLens, const void* queryLens, int lenType,

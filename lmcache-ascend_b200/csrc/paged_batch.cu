@@ -9,10 +9,9 @@
 // request), so every CTA computes them for itself into shared memory: one
 // launch, no wait of one CTA for another. New pages' numbers are then read
 // from the free list and not from the table, which other CTAs may still be
-// writing. What is left is one search over the prefix sums for each group of
-// consecutive tokens and the writes of slots and positions, so a large batch
-// is bound by those writes and a small one by one launch and three dependent
-// loads (lengths, prefix sums, page).
+// writing; the thread that has a new page's first token writes it there. What is
+// left is one search over the prefix sums for each group of consecutive tokens
+// and the writes of slots and positions.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -37,6 +36,7 @@ struct BatchParams {
   int32_t* table;
   int64_t table_stride;
   int32_t table_cols;
+  int32_t row_tokens;  // table_cols * block size
   const int32_t* free_blocks;
   int32_t num_free;
   FastDiv div_block;
@@ -66,13 +66,10 @@ __device__ __forceinline__ int32_t clamp31(int64_t v) {
   return v > INT_MAX ? INT_MAX : static_cast<int32_t>(v);
 }
 
-// Pages that `tokens` tokens fill, at most the table's width.
-__device__ __forceinline__ int32_t pages_of(int64_t tokens, const FastDiv& d, int32_t cols) {
-  // tokens < 2^32: the quotient of tokens - 1 in two steps would lose nothing,
-  // but a clamp to the largest table first keeps the numerator below 2^31.
-  const int64_t cap = static_cast<int64_t>(cols) * d.d;
-  if (tokens >= cap) return cols;
-  return tokens == 0 ? 0 : static_cast<int32_t>(d.div(static_cast<uint32_t>(tokens - 1))) + 1;
+// Pages that `tokens` (< 2^32) tokens fill, at most the table's width.
+__device__ __forceinline__ int32_t pages_of(uint32_t tokens, const BatchParams& p) {
+  if (tokens >= static_cast<uint32_t>(p.row_tokens)) return p.table_cols;
+  return tokens == 0 ? 0 : static_cast<int32_t>(p.div_block.div(tokens - 1)) + 1;
 }
 
 // Index of the last entry <= key in ascending a[0..n) (a[0] <= key).
@@ -122,8 +119,7 @@ __global__ void __launch_bounds__(kBatchThreads) build_slot_mapping_kernel(const
     if (b < B) {
       ctx = load_len(p.context_lens, p.len64, b, p.status);
       fresh = load_len(p.query_lens, p.len64, b, p.status);
-      need = pages_of(static_cast<int64_t>(ctx) + fresh, p.div_block, p.table_cols) -
-             pages_of(ctx, p.div_block, p.table_cols);
+      need = pages_of(static_cast<uint32_t>(ctx) + fresh, p) - pages_of(ctx, p);
     }
     uint32_t tok = fresh, page = need;
     warp_sums(tok, page, lane);
@@ -173,80 +169,91 @@ __global__ void __launch_bounds__(kBatchThreads) build_slot_mapping_kernel(const
   const int64_t stride = static_cast<int64_t>(gridDim.x) * threads;
   const int64_t me = static_cast<int64_t>(blockIdx.x) * threads + tid;
 
-  // New table entries, one a thread.
-  for (int64_t e = me; e < total_page; e += stride) {
-    const int r = last_le(s_first, B, static_cast<int32_t>(e));
-    const int32_t col = pages_of(s_ctx[r], p.div_block, p.table_cols) +
-                        static_cast<int32_t>(e - s_first[r]);
-    // Inside the row by construction; the test also covers sums that stopped.
-    if (col < p.table_cols) {
-      p.table[r * p.table_stride + col] = e < p.num_free ? p.free_blocks[e] : -1;
+  // The page of block `blk` of request r, from the table where the request had
+  // it and else from the free list.
+  const uint32_t size = p.div_block.d;
+  const auto page_of = [&](int r, uint32_t ctx, uint32_t blk) {
+    if (blk * size < ctx) return p.table[r * p.table_stride + blk];
+    const uint32_t f = s_first[r] + (blk - pages_of(ctx, p));
+    return f < static_cast<uint32_t>(p.num_free) ? p.free_blocks[f] : -1;
+  };
+  const auto slot_at = [&](int32_t page, uint32_t off) {
+    const int64_t at = static_cast<int64_t>(page) * size + off;
+    if (page < 0) return static_cast<SlotT>(-1);
+    if (sizeof(SlotT) == 4 && at > INT_MAX) {
+      raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
+      return static_cast<SlotT>(-1);
     }
-  }
+    return static_cast<SlotT>(at);
+  };
+  // The token at a new page's start enters the page in the table.
+  const auto enter = [&](int r, uint32_t ctx, uint32_t blk, uint32_t off, int32_t page) {
+    if (off == 0 && blk * size >= ctx) p.table[r * p.table_stride + blk] = page;
+  };
 
-  // Slots and positions, kTokensPerThread consecutive tokens a thread.
+  // kTokensPerThread consecutive tokens a thread.
   SlotT* slots = static_cast<SlotT*>(p.slots);
   SlotT* positions = static_cast<SlotT*>(p.positions);
-  const int64_t row_tokens = static_cast<int64_t>(p.table_cols) * p.div_block.d;
   for (int64_t t0 = me * kTokensPerThread; t0 < p.num_tokens; t0 += stride * kTokensPerThread) {
-    alignas(16) SlotT slot[kTokensPerThread], position[kTokensPerThread];
+    const int32_t t = static_cast<int32_t>(t0);
     int r = 0;
-    int32_t r_start = 0, r_end = 0, r_ctx = 0, r_has = 0;  // of request r, tokens [start, end)
-    int32_t blk = -1, page = -1;
-#pragma unroll
-    for (int k = 0; k < kTokensPerThread; ++k) {
-      const int32_t t = static_cast<int32_t>(t0) + k;
-      slot[k] = -1;
-      position[k] = 0;
-      if (t >= total_tok) continue;
-      if (t >= r_end) {
-        r = last_le(s_start, B, t);
-        r_start = s_start[r];
-        r_end = r + 1 < B ? s_start[r + 1] : total_tok;
-        r_ctx = s_ctx[r];
-        r_has = pages_of(r_ctx, p.div_block, p.table_cols);
-        blk = -1;
-      }
-      const int64_t pos = static_cast<int64_t>(r_ctx) + (t - r_start);
-      position[k] = static_cast<SlotT>(pos);
-      if (pos >= row_tokens) {
-        raise_flag(p.status, LMCB_DEVICE_FLAG_PAGES_EXHAUSTED);  // beyond the table's row
-        continue;
-      }
-      const int32_t b = static_cast<int32_t>(p.div_block.div(static_cast<uint32_t>(pos)));
-      if (b != blk) {
-        blk = b;
-        if (blk < r_has) {
-          page = p.table[r * p.table_stride + blk];
-        } else {
-          const int64_t f = static_cast<int64_t>(s_first[r]) + (blk - r_has);
-          page = f < p.num_free ? p.free_blocks[f] : -1;
-        }
-      }
-      if (page < 0) continue;
-      const int64_t at = static_cast<int64_t>(page) * p.div_block.d +
-                         (pos - static_cast<int64_t>(blk) * p.div_block.d);
-      if (sizeof(SlotT) == 4 && at > INT_MAX) {
-        raise_flag(p.status, LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE);
-        continue;
-      }
-      slot[k] = static_cast<SlotT>(at);
+    int32_t r_end = 0;
+    uint32_t ctx = 0, pos = 0;
+    if (t < total_tok) {
+      r = last_le(s_start, B, t);
+      r_end = r + 1 < B ? s_start[r + 1] : total_tok;
+      ctx = s_ctx[r];
+      pos = ctx + static_cast<uint32_t>(t - s_start[r]);
     }
-    if (p.aligned && t0 + kTokensPerThread <= p.num_tokens) {
+    if (p.aligned && size >= kTokensPerThread && t + kTokensPerThread <= r_end &&
+        pos + kTokensPerThread <= static_cast<uint32_t>(p.row_tokens)) {
+      // of one request and inside its row: one page, or the end of one and the
+      // start of the next
+      alignas(16) SlotT slot[kTokensPerThread], position[kTokensPerThread];
+      const uint32_t blk = p.div_block.div(pos), off = pos - blk * size;
+      const int32_t page = page_of(r, ctx, blk);
+      enter(r, ctx, blk, off, page);
+      const uint32_t in_page = size - off;
+      int32_t after = -1;
+      if (in_page < kTokensPerThread) {
+        after = page_of(r, ctx, blk + 1);
+        enter(r, ctx, blk + 1, 0, after);
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kTokensPerThread; ++k) {
+        slot[k] = k < in_page ? slot_at(page, off + k) : slot_at(after, k - in_page);
+        position[k] = static_cast<SlotT>(pos + k);
+      }
       constexpr int kVecs = sizeof(slot) / 16;
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
         reinterpret_cast<uint4*>(slots + t0)[v] = reinterpret_cast<const uint4*>(slot)[v];
         reinterpret_cast<uint4*>(positions + t0)[v] = reinterpret_cast<const uint4*>(position)[v];
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kTokensPerThread; ++k) {
-        if (t0 + k < p.num_tokens) {
-          slots[t0 + k] = slot[k];
-          positions[t0 + k] = position[k];
+      continue;
+    }
+#pragma unroll 1
+    for (int32_t u = t; u < t + kTokensPerThread && u < p.num_tokens; ++u) {
+      SlotT slot = -1, position = 0;
+      if (u < total_tok) {
+        if (u >= r_end) {
+          r = last_le(s_start, B, u);
+          r_end = r + 1 < B ? s_start[r + 1] : total_tok;
+          ctx = s_ctx[r];
+        }
+        pos = ctx + static_cast<uint32_t>(u - s_start[r]);
+        position = static_cast<SlotT>(pos);
+        if (pos < static_cast<uint32_t>(p.row_tokens)) {
+          const uint32_t blk = p.div_block.div(pos), off = pos - blk * size;
+          const int32_t page = page_of(r, ctx, blk);
+          enter(r, ctx, blk, off, page);
+          slot = slot_at(page, off);
+        } else {
+          raise_flag(p.status, LMCB_DEVICE_FLAG_PAGES_EXHAUSTED);  // beyond the table's row
         }
       }
+      slots[u] = slot;
+      positions[u] = position;
     }
   }
 }
@@ -293,6 +300,7 @@ int lmcb_build_slot_mapping(const void* contextLens, const void* queryLens, int 
   p.table = blockTable;
   p.table_stride = tableStride;
   p.table_cols = tableCols;
+  p.row_tokens = tableCols * blockSize;
   p.free_blocks = freeBlocks;
   p.num_free = static_cast<int32_t>(numFree);
   p.div_block = lmcb::FastDiv(static_cast<uint32_t>(blockSize));
@@ -310,7 +318,7 @@ int lmcb_build_slot_mapping(const void* contextLens, const void* queryLens, int 
       (numTokens + lmcb::kTokensPerThread - 1) / lmcb::kTokensPerThread;
   const int threads = groups <= 256 && numRequests <= 256 ? 256 : lmcb::kBatchThreads;
   const int64_t want = (groups + threads - 1) / threads;
-  const int64_t most = lmcb::current_sm_count();
+  const int64_t most = lmcb::current_sm_count() * 2;
   const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
   const size_t smem = static_cast<size_t>(numRequests) * 12;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -460,168 +460,255 @@ __device__ __forceinline__ int64_t qk_position(const QkNormParams& p, int64_t to
 }
 
 constexpr int kQkThreads = 256;
-constexpr int kQkRowsInFlight = 2;
 
 // kLanes lanes share a head row; a lane holds two 16-byte vectors of it: for
 // neox a vector of the first rotary half and its partner in the second (so a
 // pair never leaves its lane), else two vectors of adjacent pairs; lanes behind
 // the rotated part hold two vectors of the rest. A warp takes one token and a
-// run of its heads (q heads, then k heads), 32 / kLanes heads a pass: the
-// cos/sin values a lane needs are the same for every head, so it loads them
-// once for the run.
-template <typename T, bool kNeox, int kLanes>
-__global__ void __launch_bounds__(kQkThreads, 3)
-qk_norm_rope_vec_kernel(const QkNormParams p, const uint32_t num_items, const FastDiv div_runs,
-                        const int heads_per_run) {
-  constexpr int E = 16 / sizeof(T);
-  constexpr int kHeadsPerPass = 32 / kLanes;
-  using V = Vec16<T>;
-  const int lane = threadIdx.x % 32;
-  const int l = lane % kLanes;
-  const int sub = lane / kLanes;
-  const int D = p.head_size, rot = p.rot_dim;
-  const bool active = l * 2 * E < D;
-  // the two vectors of this lane, and whether they are rotated
+// run of its heads (q heads, then k heads), 32 / kLanes heads a step. With r = 1 / sqrt(mean + eps), a pair's results are
+//   y1 = r (x1 (w1 cos) - x2 (w2 sin)),  y2 = r (x2 (w2 cos) + x1 (w1 sin)),
+// (cos = 1 and sin = 0 where nothing is rotated), and the four products with
+// the weights are the same for every q head of the token, and every k head: a
+// lane makes them once for the run.
+template <typename T>
+struct QkFactors {
+  static constexpr int E = 16 / sizeof(T);  // pairs of a lane
+  float c1[E], s2[E], c2[E], s1[E];         // w1 cos, w2 sin, w2 cos, w1 sin
+};
+
+// A lane's two vectors of a row: their first elements, and whether they are
+// rotated.
+struct QkLane {
   int e0, e1;
   bool turn0, turn1;
+};
+
+// Where the factors of a row come from: weights (NULL: none) and a row [cos |
+// sin] of `half` values each.
+struct QkSource {
+  const void* weight;
+  int weight_type;
+  const void* cache;
+  int cache_type;
+  int64_t row;
+  int half;
+};
+
+template <typename T, bool kNeox>
+__device__ __forceinline__ void qk_factors(const QkSource& src, const QkLane& ln,
+                                           QkFactors<T>& f) {
+  constexpr int E = 16 / sizeof(T);
+  float wa[E], wb[E], cs[E], sn[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) wa[j] = wb[j] = cs[j] = 1.0f, sn[j] = 0.0f;
+  if (src.weight != nullptr) {
+    load_run_typed<E>(src.weight, src.weight_type, ln.e0, wa);
+    load_run_typed<E>(src.weight, src.weight_type, ln.e1, wb);
+  }
+  if constexpr (kNeox) {
+    if (ln.turn0) {
+      load_run_typed<E>(src.cache, src.cache_type, src.row + ln.e0, cs);
+      load_run_typed<E>(src.cache, src.cache_type, src.row + src.half + ln.e0, sn);
+    }
+  } else {
+    float c[E / 2], s[E / 2];
+    if (ln.turn0) {
+      load_run_typed<E / 2>(src.cache, src.cache_type, src.row + ln.e0 / 2, c);
+      load_run_typed<E / 2>(src.cache, src.cache_type, src.row + src.half + ln.e0 / 2, s);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) cs[j] = c[j], sn[j] = s[j];
+    }
+    if (ln.turn1) {
+      load_run_typed<E / 2>(src.cache, src.cache_type, src.row + ln.e1 / 2, c);
+      load_run_typed<E / 2>(src.cache, src.cache_type, src.row + src.half + ln.e1 / 2, s);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) cs[E / 2 + j] = c[j], sn[E / 2 + j] = s[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    float w1, w2;
+    if constexpr (kNeox) {
+      w1 = wa[j];
+      w2 = wb[j];
+    } else {
+      w1 = j < E / 2 ? wa[2 * j] : wb[2 * j - E];
+      w2 = j < E / 2 ? wa[2 * j + 1] : wb[2 * j - E + 1];
+    }
+    f.c1[j] = w1 * cs[j];
+    f.s1[j] = w1 * sn[j];
+    f.c2[j] = w2 * cs[j];
+    f.s2[j] = w2 * sn[j];
+  }
+}
+
+template <bool kNeox, int E>
+__device__ __forceinline__ QkLane qk_lane(int l, int rot) {
+  QkLane ln;
   if constexpr (kNeox) {
     const int pairs = rot / 2 / E;  // lanes that hold rotated vectors
-    turn0 = turn1 = l < pairs;
-    e0 = l < pairs ? l * E : rot + (l - pairs) * 2 * E;
-    e1 = l < pairs ? rot / 2 + l * E : e0 + E;
+    ln.turn0 = ln.turn1 = l < pairs;
+    ln.e0 = l < pairs ? l * E : rot + (l - pairs) * 2 * E;
+    ln.e1 = l < pairs ? rot / 2 + l * E : ln.e0 + E;
   } else {
-    e0 = l * 2 * E;
-    e1 = e0 + E;
-    turn0 = e0 < rot;
-    turn1 = e1 < rot;
+    ln.e0 = l * 2 * E;
+    ln.e1 = ln.e0 + E;
+    ln.turn0 = ln.e0 < rot;
+    ln.turn1 = ln.e1 < rot;
   }
-  const int all_heads = p.heads[0] + p.heads[1];
+  return ln;
+}
+
+// One head row, in a lane's two vectors: x becomes the result. All lanes of a
+// warp take part; `live` lanes hold something.
+template <typename T, bool kNeox, int kLanes>
+__device__ __forceinline__ void qk_row(Vec16<T> (&x)[2], const QkFactors<T>& f, float mean,
+                                       float eps, bool live) {
+  constexpr int E = 16 / sizeof(T);
+  float x1[E], x2[E];  // the pairs
+  float ss = 0.0f;
+  if (live) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if constexpr (kNeox) {
+        x1[j] = to_f(x[0].v[j]);
+        x2[j] = to_f(x[1].v[j]);
+      } else {
+        x1[j] = to_f(j < E / 2 ? x[0].v[2 * j] : x[1].v[2 * j - E]);
+        x2[j] = to_f(j < E / 2 ? x[0].v[2 * j + 1] : x[1].v[2 * j - E + 1]);
+      }
+      ss = fmaf(x1[j], x1[j], ss);
+      ss = fmaf(x2[j], x2[j], ss);
+    }
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (!live) return;
+  const float r = rsqrtf(fmaf(ss, mean, eps));
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const T y1 = from_f<T>(r * fmaf(x1[j], f.c1[j], -(x2[j] * f.s2[j])));
+    const T y2 = from_f<T>(r * fmaf(x2[j], f.c2[j], x1[j] * f.s1[j]));
+    if constexpr (kNeox) {
+      x[0].v[j] = y1;
+      x[1].v[j] = y2;
+    } else if (j < E / 2) {
+      x[0].v[2 * j] = y1;
+      x[0].v[2 * j + 1] = y2;
+    } else {
+      x[1].v[2 * j - E] = y1;
+      x[1].v[2 * j - E + 1] = y2;
+    }
+  }
+}
+
+// An item is a token and a run of its heads. The factors' registers leave an SM
+// 16 warps, and a step is 1 KB a warp: less than memory has to have under way.
+// So a lane brings its vectors of the next kQkAhead steps, of the next items
+// too, by asynchronous copies into places of its own in shared memory, which
+// nobody else reads: there is nothing to wait for but its own copies.
+// Measured for 16384 tokens of 64 + 8 heads of 128 (bf16, 604 MB): 147 us with
+// two steps ahead in registers, and with a ring of whole tokens by bulk copies.
+constexpr int kQkAhead = 6;
+
+// 16 bytes, asynchronously.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <typename T, bool kNeox, int kLanes>
+__global__ void __launch_bounds__(kQkThreads, 2)
+qk_norm_rope_vec_kernel(const __grid_constant__ QkNormParams p, const uint32_t num_items,
+                        const FastDiv div_runs, const int heads_per_run) {
+  constexpr int E = 16 / sizeof(T);
+  constexpr int kHeadsPerStep = 32 / kLanes;
+  using V = Vec16<T>;
+  __shared__ V ring[kQkAhead][2][kQkThreads];
+  const int lane = threadIdx.x % 32;
+  const int D = p.head_size;
+  const QkLane ln = qk_lane<kNeox, E>(lane % kLanes, p.rot_dim);
+  const bool active = lane % kLanes * 2 * E < D;
+  const int q_heads = p.heads[0], all_heads = p.heads[0] + p.heads[1];
+  const float mean = 1.0f / static_cast<float>(D);
   const uint32_t warps = gridDim.x * (kQkThreads / 32);
-  for (uint32_t item = blockIdx.x * (kQkThreads / 32) + threadIdx.x / 32; item < num_items;
-       item += warps) {
+  const uint32_t first = blockIdx.x * (kQkThreads / 32) + threadIdx.x / 32;
+  const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&ring[0][0][threadIdx.x]));
+
+  // The step that is brought next: its item, and this lane's head.
+  uint32_t far_item = first;
+  int far_h = 0, far_last = 0;
+  const T *far_q = nullptr, *far_k = nullptr;
+  const auto far_start = [&]() {
+    if (far_item >= num_items) return;
+    const uint32_t t = div_runs.div(far_item);
+    const int h_first = static_cast<int>(far_item - t * div_runs.d) * heads_per_run;
+    far_h = h_first + lane / kLanes;
+    far_last = min(h_first + heads_per_run, all_heads);
+    far_q = static_cast<const T*>(p.in[0]) + t * p.in_stride[0];
+    far_k = static_cast<const T*>(p.in[1]) + t * p.in_stride[1] -
+            static_cast<int64_t>(q_heads) * D;
+  };
+  const auto bring = [&](int slot) {
+    if (far_item < num_items) {
+      if (far_h < far_last && active) {
+        const T* row = (far_h < q_heads ? far_q : far_k) + static_cast<int64_t>(far_h) * D;
+        const uint32_t to = mine + slot * static_cast<uint32_t>(sizeof(ring[0]));
+        copy_async16(to, row + ln.e0);
+        copy_async16(to + static_cast<uint32_t>(sizeof(ring[0][0])), row + ln.e1);
+      }
+      far_h += kHeadsPerStep;
+      if (far_h - lane / kLanes >= far_last) {  // uniform: the item's last step
+        far_item += warps;
+        far_start();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  far_start();
+#pragma unroll
+  for (int u = 0; u + 1 < kQkAhead; ++u) bring(u);
+
+  int slot = 0;
+  int64_t next_pos = first < num_items ? qk_position(p, div_runs.div(first)) : 0;
+  for (uint32_t item = first; item < num_items; item += warps) {
     const uint32_t t = div_runs.div(item);
     const int h_first = static_cast<int>(item - t * div_runs.d) * heads_per_run;
     const int h_last = min(h_first + heads_per_run, all_heads);
-    const int64_t pos = qk_position(p, t);
-    float cs[E], sn[E];  // neox: one run of E; else E / 2 for each vector
-    for (int h0 = h_first; h0 < h_last; h0 += kHeadsPerPass * kQkRowsInFlight) {
-      V x[kQkRowsInFlight][2];
-#pragma unroll
-      for (int u = 0; u < kQkRowsInFlight; ++u) {
-        const int h = h0 + u * kHeadsPerPass + sub;
-        if (h < h_last && active) {
-          const int which = h >= p.heads[0];
-          const T* row = static_cast<const T*>(p.in[which]) +
-                         static_cast<int64_t>(t) * p.in_stride[which] +
-                         static_cast<int64_t>(h - (which ? p.heads[0] : 0)) * D;
-          x[u][0] = *reinterpret_cast<const V*>(row + e0);
-          x[u][1] = *reinterpret_cast<const V*>(row + e1);
-        }
+    const int64_t pos = next_pos;
+    if (item + warps < num_items) next_pos = qk_position(p, div_runs.div(item + warps));
+    const bool ok = pos >= 0 && pos < p.max_position;
+    if (!ok && lane == 0 && h_first == 0) {
+      raise_flag(p.status, LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE);
+    }
+    QkFactors<T> f;
+    int made_for = -1;  // q (0) or k (1) heads
+    for (int h0 = h_first; h0 < h_last; h0 += kHeadsPerStep) {
+      bring(slot == 0 ? kQkAhead - 1 : slot - 1);
+      const int h = h0 + lane / kLanes;
+      const bool live = h < h_last && active && ok;
+      const int which = h >= q_heads;
+      if (live && which != made_for) {
+        const QkSource src{which ? p.weight[1] : p.weight[0],
+                           which ? p.weight_type[1] : p.weight_type[0], p.cache, p.cache_type,
+                           pos * p.rot_dim, p.rot_dim / 2};
+        qk_factors<T, kNeox>(src, ln, f);
+        made_for = which;
       }
-      if (h0 == h_first) {
-        if (pos < 0 || pos >= p.max_position) {
-          if (lane == 0 && h_first == 0) {
-            raise_flag(p.status, LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE);
-          }
-          break;  // uniform: the token's rows are left as they were
-        }
-        const int64_t row = pos * rot;
-        if (kNeox) {
-          if (active && turn0) {
-            load_run_typed<E>(p.cache, p.cache_type, row + e0, cs);
-            load_run_typed<E>(p.cache, p.cache_type, row + rot / 2 + e0, sn);
-          }
-        } else {
-          float c2[E / 2], s2[E / 2];
-          if (active && turn0) {
-            load_run_typed<E / 2>(p.cache, p.cache_type, row + e0 / 2, c2);
-            load_run_typed<E / 2>(p.cache, p.cache_type, row + rot / 2 + e0 / 2, s2);
-#pragma unroll
-            for (int j = 0; j < E / 2; ++j) cs[j] = c2[j], sn[j] = s2[j];
-          }
-          if (active && turn1) {
-            load_run_typed<E / 2>(p.cache, p.cache_type, row + e1 / 2, c2);
-            load_run_typed<E / 2>(p.cache, p.cache_type, row + rot / 2 + e1 / 2, s2);
-#pragma unroll
-            for (int j = 0; j < E / 2; ++j) cs[E / 2 + j] = c2[j], sn[E / 2 + j] = s2[j];
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kQkRowsInFlight; ++u) {
-        const int h = h0 + u * kHeadsPerPass + sub;
-        const bool live = h < h_last && active;
-        const int which = h >= p.heads[0];
-        float a[E], b[E];
-        float ss = 0.0f;
-        if (live) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            a[j] = to_f(x[u][0].v[j]);
-            b[j] = to_f(x[u][1].v[j]);
-            ss = fmaf(a[j], a[j], ss);
-            ss = fmaf(b[j], b[j], ss);
-          }
-        }
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!live) continue;
-        const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
-        if (p.weight[which] != nullptr) {
-          float wa[E], wb[E];
-          load_run_typed<E>(p.weight[which], p.weight_type[which], e0, wa);
-          load_run_typed<E>(p.weight[which], p.weight_type[which], e1, wb);
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            a[j] = a[j] * inv * wa[j];
-            b[j] = b[j] * inv * wb[j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            a[j] *= inv;
-            b[j] *= inv;
-          }
-        }
-        if constexpr (kNeox) {
-          if (turn0) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              float y1, y2;
-              rotate_pair(a[j], b[j], cs[j], sn[j], y1, y2);
-              a[j] = y1;
-              b[j] = y2;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < E / 2; ++j) {
-            float y1, y2;
-            if (turn0) {
-              rotate_pair(a[2 * j], a[2 * j + 1], cs[j], sn[j], y1, y2);
-              a[2 * j] = y1;
-              a[2 * j + 1] = y2;
-            }
-            if (turn1) {
-              rotate_pair(b[2 * j], b[2 * j + 1], cs[E / 2 + j], sn[E / 2 + j], y1, y2);
-              b[2 * j] = y1;
-              b[2 * j + 1] = y2;
-            }
-          }
-        }
-        T* row = static_cast<T*>(p.out[which]) + static_cast<int64_t>(t) * p.out_stride[which] +
-                 static_cast<int64_t>(h - (which ? p.heads[0] : 0)) * D;
-        V ya, yb;
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          ya.v[j] = from_f<T>(a[j]);
-          yb.v[j] = from_f<T>(b[j]);
-        }
-        *reinterpret_cast<V*>(row + e0) = ya;
-        *reinterpret_cast<V*>(row + e1) = yb;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kQkAhead - 1) : "memory");
+      V x[2] = {ring[slot][0][threadIdx.x], ring[slot][1][threadIdx.x]};
+      if (++slot == kQkAhead) slot = 0;
+      qk_row<T, kNeox, kLanes>(x, f, mean, p.eps, live);
+      if (live) {
+        T* row = which ? static_cast<T*>(p.out[1]) + t * p.out_stride[1] +
+                             static_cast<int64_t>(h - q_heads) * D
+                       : static_cast<T*>(p.out[0]) + t * p.out_stride[0] +
+                             static_cast<int64_t>(h) * D;
+        *reinterpret_cast<V*>(row + ln.e0) = x[0];
+        *reinterpret_cast<V*>(row + ln.e1) = x[1];
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The same for every other size and alignment: a warp a head row, element by
@@ -698,19 +785,17 @@ bool qk_vec_ok(const QkNormParams& p, bool neox) {
 
 template <typename T, bool kNeox, int kLanes>
 void launch_qk_vec(const QkNormParams& p, cudaStream_t stream) {
-  constexpr int kPerStep = 32 / kLanes * kQkRowsInFlight;
   const int heads = p.heads[0] + p.heads[1];
-  // A warp's run of heads: as few as one step while that leaves warps idle,
-  // all of them once the tokens alone fill the GPU.
-  const int64_t slots = static_cast<int64_t>(current_sm_count()) * 24;
-  int64_t runs = (heads + kPerStep - 1) / kPerStep;
-  while (runs > 1 && p.num_tokens * (runs / 2) >= slots) runs /= 2;
-  int per_run = static_cast<int>((heads + runs - 1) / runs);
-  per_run = (per_run + kPerStep - 1) / kPerStep * kPerStep;
+  const int64_t sms = current_sm_count();
+  // A step a warp while warps are left, then longer runs.
+  const int64_t steps = (heads + 32 / kLanes - 1) / (32 / kLanes);
+  int64_t runs = steps;
+  while (runs > 1 && p.num_tokens * (runs / 2) >= sms * 16) runs /= 2;
+  int per_run = static_cast<int>((steps + runs - 1) / runs) * (32 / kLanes);
   runs = (heads + per_run - 1) / per_run;
   const int64_t items = p.num_tokens * runs;
   const int64_t want = (items + kQkThreads / 32 - 1) / (kQkThreads / 32);
-  const int64_t most = static_cast<int64_t>(current_sm_count()) * 8;
+  const int64_t most = sms * 2;
   qk_norm_rope_vec_kernel<T, kNeox, kLanes>
       <<<static_cast<unsigned>(want < most ? want : most), kQkThreads, 0, stream>>>(
           p, static_cast<uint32_t>(items), FastDiv(static_cast<uint32_t>(runs)), per_run);

@@ -239,6 +239,36 @@ def test_qk_packed_and_in_place(offset, in_place):
                     seed=offset)
 
 
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_qk_few_and_many_tokens(neox, dtype):
+    """Few and many tokens, whole and partial rotation, packed and in place."""
+    for t, hq, hk, d, rot in ((1, 3, 1, 128, 128), (700, 5, 2, 64, 32), (901, 4, 1, 80, 80),
+                              (300, 2, 2, 256, 0), (1300, 12, 3, 128, 96), (40, 0, 2, 128, 128),
+                              (650, 2, 0, 64, 64), (7, 40, 8, 512, 512)):
+        qk_case(t, hq, hk, d, rot, neox, dtype, seed=t)
+        qk_case(t, hq, hk, d, rot, neox, dtype, packed=True, in_place=True, offset=8, seed=t,
+                wdtype=torch.float32, cdtype=torch.bfloat16, pdtype=torch.int32)
+
+
+def test_qk_many_bad_positions():
+    t = 1000
+    cache = cos_sin(64, 128).to(DEV)
+    q = torch.randn(t, 3, 128, device=DEV).bfloat16()
+    k = torch.randn(t, 2, 128, device=DEV).bfloat16()
+    pos = torch.randint(0, 64, (t,), device=DEV)
+    bad = torch.randperm(t, device=DEV)[:300]
+    pos[bad] = torch.where(bad % 2 == 0, -1, 1 << 40)
+    qo, ko = torch.full_like(q, 3), torch.full_like(k, 3)
+    c_ops.qk_norm_rope(q, k, None, None, pos, cache, 1e-6, True, qo, ko)
+    assert c_ops.device_status(0) == FLAGS.LMCB_DEVICE_FLAG_POSITION_OUT_OF_RANGE
+    good = torch.ones(t, dtype=torch.bool, device=DEV)
+    good[bad] = False
+    assert bool((qo[~good] == 3).all()) and bool((ko[~good] == 3).all())
+    check_qk(qo[good], q[good], None, pos[good], cache, 1e-6, True)
+    check_qk(ko[good], k[good], None, pos[good], cache, 1e-6, True)
+
+
 @pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("cdtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_qk_weight_cache_and_position_types(wdtype, cdtype):
