@@ -163,33 +163,69 @@ __device__ __forceinline__ void row_range(const Eight<T>& x, bool active, float&
 // multiply-add by 16^i puts it in its place, and what the eight exponent fields
 // add up to is one constant. Only an element that lies that close to the border
 // between two codes is taken again, in 64 bits: three in a hundred thousand.
-__device__ __forceinline__ uint32_t word_of(const float (&v)[8], float z, float s) {
-  constexpr float kMagic = 12582912.0f;
+struct Coder {
+  float inv, shift, sure;  // 1 / (15 s), -z / (15 s), and how close is too close
+
+  __device__ __forceinline__ Coder(float z, float s) {
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.0f * s));
+    shift = -z * inv;
+    sure = 0.5f - fmaf(fabsf(shift), 15.0f, 8.0f) * 4.7683716e-7f;
+  }
+};
+
+constexpr float kMagic = 12582912.0f;
+
+// Two fp32 values an instruction.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// `off` grows to how far the word's elements are from their codes, in steps.
+__device__ __forceinline__ uint32_t word_of(const float (&v)[8], const Coder& c, float& off) {
   constexpr uint32_t kBias = 0x4B400000u * 0x11111111u;
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.0f * s));
-  const float shift = -z * inv;
-  const float sure = 0.5f - fmaf(fabsf(shift), 15.0f, 8.0f) * 4.7683716e-7f;
+  const uint64_t magic = pack2(kMagic, kMagic), fifteen = pack2(15.0f, 15.0f);
+  const uint64_t minus = pack2(-1.0f, -1.0f);
   uint32_t word = 0;
-  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t y = pack2(__saturatef(fmaf(v[i], c.inv, c.shift)),
+                             __saturatef(fmaf(v[i + 1], c.inv, c.shift)));
+    const uint64_t r = fma2(y, fifteen, magic);
+    const float2 away = unpack2(fma2(y, fifteen, fma2(r, minus, magic)));
+    off = fmaxf(off, fmaxf(fabsf(away.x), fabsf(away.y)));
+    const float2 bits = unpack2(r);
+    word += __float_as_uint(bits.x) << (4 * i);
+    word += __float_as_uint(bits.y) << (4 * i + 4);
+  }
+  return word - kBias;
+}
+
+// The word again, with the elements that are too close to a border in 64 bits.
+__device__ __noinline__ uint32_t exact_word(float v0, float v1, float v2, float v3, float v4,
+                                            float v5, float v6, float v7, uint32_t word, float z,
+                                            float s) {
+  const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+  const Coder c(z, s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = __saturatef(fmaf(v[i], inv, shift));
-    const float r = fmaf(y, 15.0f, kMagic);
-    off = fmaxf(off, fabsf(fmaf(y, 15.0f, kMagic - r)));
-    word += __float_as_uint(r) << (4 * i);
-  }
-  word -= kBias;
-  if (off >= sure) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __saturatef(fmaf(v[i], inv, shift));
-      if (fabsf(fmaf(y, 15.0f, kMagic - fmaf(y, 15.0f, kMagic))) >= sure) {
-        const double q =
-            (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
-        const uint32_t code = static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
-        word = (word & ~(15u << (4 * i))) | (code << (4 * i));
-      }
+    const float y = __saturatef(fmaf(v[i], c.inv, c.shift));
+    if (fabsf(fmaf(y, 15.0f, kMagic - fmaf(y, 15.0f, kMagic))) >= c.sure) {
+      const double q =
+          (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
+      const uint32_t code = static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
+      word = (word & ~(15u << (4 * i))) | (code << (4 * i));
     }
   }
   return word;
@@ -230,9 +266,63 @@ __device__ __forceinline__ Item item_of(const Kv4Params& p, uint64_t at, bool fl
   return it;
 }
 
+// The head rows x of a group into the cache. kWild: some row of the warp holds
+// NaN or a value beyond the fp16 range.
+template <typename T, int kGroup, int kHeads, bool kFull, bool kWild>
+__device__ __forceinline__ void store_rows(const Eight<T> (&x)[kHeads], float (&lo)[kHeads],
+                                           float (&hi)[kHeads], bool active, int count, int lane,
+                                           int words, int32_t* codes, int32_t* params) {
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(x[k].v[i]);
+    if constexpr (kWild) {
+      lo[k] = INFINITY;
+      hi[k] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = finite_half_range(v[i]);
+        if (active) {
+          lo[k] = fminf(lo[k], v[i]);
+          hi[k] = fmaxf(hi[k], v[i]);
+        }
+      }
+#pragma unroll
+      for (int o = kGroup / 2; o > 0; o >>= 1) {
+        lo[k] = fminf(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], o));
+        hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
+      }
+    }
+    // The fp32 quotient by 15, rounded once: that of 24 bits by 15 is never closer
+    // than 2^-29 of itself to a border between two fp32 numbers, and the product
+    // in 64 bits is off by 2^-52.
+    const float span = static_cast<float>(static_cast<double>(hi[k] - lo[k]) * (1.0 / 15.0));
+    const __half sh = __float2half_rn(span);
+    // + 0: a zero of either sign is kept as +0, so equal rows have equal words
+    const float z = __half2float(__float2half_rn(lo[k])) + 0.0f;
+    const float s = __half2float(sh);
+    const Coder c(z, s);
+    float off = 0.0f;
+    uint32_t word = word_of(v, c, off);
+    if (off >= c.sure) word = exact_word(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], word, z, s);
+    if (s == 0.0f) word = 0;  // one value only: z
+    if ((kFull ? count > 0 : k < count) && active) {
+      codes[k * words] = static_cast<int32_t>(word);
+      if (lane == 0) {
+        params[k] = static_cast<int32_t>(
+            static_cast<uint32_t>(__half_as_ushort(sh)) |
+            (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(z))) << 16));
+      }
+    }
+  }
+}
+
 // kGroup lanes share a head row (D <= 8 * kGroup).
-template <typename T, int kGroup, int kHeads, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Params p) {
+// kFull: kHeads divides the heads.
+template <typename T, int kGroup, int kHeads, bool kVec, bool kFull>
+__global__ void __launch_bounds__(kThreads, 4)
+kv4_store_kernel(const __grid_constant__ Kv4Params p) {
   const int lane = threadIdx.x % kGroup;
   const int D = p.head_size;
   const bool active = lane * 8 < D;
@@ -243,59 +333,36 @@ __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Params p) 
     Eight<T> x[kHeads] = {};
     if (it.count > 0 && active) {
       const T* src = static_cast<const T*>(it.half ? p.src[1] : p.src[0]) +
-                     static_cast<int64_t>(it.token) * (it.half ? p.token_stride[1] : p.token_stride[0]) +
+                     static_cast<int64_t>(it.token) *
+                         (it.half ? p.token_stride[1] : p.token_stride[0]) +
                      static_cast<int64_t>(it.head) * D + lane * 8;
 #pragma unroll
       for (int k = 0; k < kHeads; ++k) {
-        if (k < it.count) x[k] = load8<T, kVec>(src + k * D);
+        if (kFull || k < it.count) x[k] = load8<T, kVec>(src + k * D);
       }
     }
     int32_t* row = p.cache + (it.half ? p.half_words : 0) + it.slot * p.row_words;
     int32_t* codes = row + static_cast<int64_t>(it.head) * (D / 8) + lane;
     int32_t* params = row + static_cast<int64_t>(p.num_heads) * (D / 8) + it.head;
+    float lo[kHeads], hi[kHeads];
+    bool tame = true;
 #pragma unroll
     for (int k = 0; k < kHeads; ++k) {
-      float lo, hi;
-      row_range<T, kGroup>(x[k], active, lo, hi);
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_float(x[k].v[i]);
-      if (__any_sync(0xffffffffu, !(lo >= -65504.0f && hi <= 65504.0f))) {
-        lo = INFINITY;
-        hi = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = finite_half_range(v[i]);
-          if (active) {
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
-          }
-        }
-#pragma unroll
-        for (int o = kGroup / 2; o > 0; o >>= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-      }
-      if (k < it.count && active) {
-        const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
-        // + 0: a zero of either sign is kept as +0, so equal rows have equal words
-        const float z = __half2float(__float2half_rn(lo)) + 0.0f;
-        const float s = __half2float(sh);
-        const uint32_t word = s > 0.0f ? word_of(v, z, s) : 0;
-        codes[k * (D / 8)] = static_cast<int32_t>(word);
-        if (lane == 0) {
-          params[k] = static_cast<int32_t>(
-              static_cast<uint32_t>(__half_as_ushort(sh)) |
-              (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(z))) << 16));
-        }
-      }
+      row_range<T, kGroup>(x[k], active, lo[k], hi[k]);
+      tame = tame && lo[k] >= -65504.0f && hi[k] <= 65504.0f;
+    }
+    if (__all_sync(0xffffffffu, tame)) {
+      store_rows<T, kGroup, kHeads, kFull, false>(x, lo, hi, active, it.count, lane, D / 8, codes,
+                                                  params);
+    } else {
+      store_rows<T, kGroup, kHeads, kFull, true>(x, lo, hi, active, it.count, lane, D / 8, codes,
+                                                 params);
     }
   }
 }
 
 template <typename T, int kGroup, int kHeads, bool kVec>
-__global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(kThreads) kv4_load_kernel(const __grid_constant__ Kv4Params p) {
   const int lane = threadIdx.x % kGroup;
   const int D = p.head_size;
   if (lane * 8 >= D) return;
@@ -345,7 +412,11 @@ void launch_items(Kv4Params p, bool store, cudaStream_t stream) {
   const uint64_t most = static_cast<uint64_t>(current_sm_count()) * 8;
   const unsigned grid = static_cast<unsigned>(want < most ? want : most);
   if (store) {
-    kv4_store_kernel<T, kGroup, kHeads, kVec><<<grid, kThreads, 0, stream>>>(p);
+    if (p.num_heads % kHeads == 0) {
+      kv4_store_kernel<T, kGroup, kHeads, kVec, true><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+      kv4_store_kernel<T, kGroup, kHeads, kVec, false><<<grid, kThreads, 0, stream>>>(p);
+    }
   } else {
     kv4_load_kernel<T, kGroup, kHeads, kVec><<<grid, kThreads, 0, stream>>>(p);
   }
