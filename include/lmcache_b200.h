@@ -432,10 +432,11 @@ LMCB_API int lmcb_qk_norm_rope(const void* query, const void* key, int type,
  * (word h * D / 8 + w: values 8 w ... 8 w + 7 of head h, value 8 w + j in bits
  * 4 j ... 4 j + 3), then one word a head: fp16 scale s in the low half, fp16
  * zero z in the high half. A code c stands for z + s c, with z = fp16(min),
- * s = fp16((max - min) / 15) of the head's values and the nearest code, ties
- * to even; NaN is kept as 0, values beyond the fp16 range as its ends. W is
- * that length rounded up to four words, so a 4-bit cache moves through the
- * transfers above as rows of W int32 (type LMCB_DTYPE_INT32, hiddenDims W). */
+ * s = fp16((max - min) * r), r the fp32 number nearest to 1 / 15, of the head's
+ * values and the nearest code, ties to even; NaN is kept as 0, values beyond
+ * the fp16 range as its ends. W is that length rounded up to four words, so a
+ * 4-bit cache moves through the transfers above as rows of W int32 (type
+ * LMCB_DTYPE_INT32, hiddenDims W). */
 
 /* W, or 0 for a head size that is not a multiple of 8 up to 256. */
 LMCB_API int64_t lmcb_kv4_row_words(int64_t numHeads, int64_t headSize);
@@ -459,7 +460,9 @@ LMCB_API int lmcb_kv4_load(const int32_t* kvCache, int64_t numBlocks, int64_t bl
 /* Attention of a batch over its 4-bit pages.
  *   query, out     [numQueryRows, numQueryHeads, headSize] bf16 or fp16, tokens
  *                  *TokenStride elements apart; headSize 64, 128 or 256
- *   blockTable     [batch, tableCols] int32, rows tableStride apart
+ *   blockTable     [batch, tableCols] int32, rows tableStride apart; at most 4096
+ *                  requests and 2^35 keys that the table has room for
+ *                  (LMCB_ERR_CAPACITY)
  *   seqLens        [batch] int32: tokens in the cache, the queries' own among them
  *   queryStart     [batch + 1] int32: request b's queries are rows
  *                  queryStart[b] ... queryStart[b + 1], the last of them at

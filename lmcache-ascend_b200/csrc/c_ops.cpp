@@ -697,6 +697,24 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// Whether two sets of rows [tokens, heads, head_size], dense within a token,
+// share memory. Parts of one packed projection lie in the same range of bytes
+// but not in the same columns.
+bool rows_overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  if (!overlap(a, b)) return false;
+  if (a.size(0) < 2 || b.size(0) < 2 || a.stride(0) != b.stride(0) ||
+      a.element_size() != b.element_size()) {
+    return true;
+  }
+  const int64_t esz = a.element_size(), step = a.stride(0) * esz;
+  const int64_t row_a = a.size(1) * a.size(2) * esz, row_b = b.size(1) * b.size(2) * esz;
+  int64_t apart = (static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr())) -
+                   static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data_ptr()))) %
+                  step;
+  if (apart < 0) apart += step;
+  return apart < row_a || apart + row_b > step;
+}
+
 void check_cuda(const torch::Tensor& t, const torch::Device& dev, const char* who,
                 const char* name) {
   TORCH_CHECK(t.is_cuda(), who, ": ", name, " must be a CUDA tensor");
@@ -835,18 +853,17 @@ void qk_norm_rope(const torch::Tensor& query, const torch::Tensor& key,
     weights[i] = w.data_ptr();
     weight_types[i] = to_lmcb_dtype(w.scalar_type());
   }
-  // An output is its input, element for element, or shares nothing with
-  // either input (two parts of one packed projection both count).
+  // An output is its input, element for element, or shares nothing with either
+  // input.
   const auto in_place = [](const torch::Tensor& out, const torch::Tensor& in) {
     return out.data_ptr() == in.data_ptr() && token_stride(out) == token_stride(in);
   };
   const bool q_in_place = in_place(query_out, query), k_in_place = in_place(key_out, key);
-  TORCH_CHECK(q_in_place || (!overlap(query_out, query) && !overlap(query_out, key)), who,
-              ": query_out must be query or overlap no input");
-  TORCH_CHECK(k_in_place || (!overlap(key_out, key) && !overlap(key_out, query)), who,
+  TORCH_CHECK((q_in_place || !rows_overlap(query_out, query)) && !rows_overlap(query_out, key),
+              who, ": query_out must be query or overlap no input");
+  TORCH_CHECK((k_in_place || !rows_overlap(key_out, key)) && !rows_overlap(key_out, query), who,
               ": key_out must be key or overlap no input");
-  TORCH_CHECK((q_in_place && k_in_place) || !overlap(query_out, key_out), who,
-              ": outputs overlap");
+  TORCH_CHECK(!rows_overlap(query_out, key_out), who, ": outputs overlap");
   const c10::cuda::CUDAGuard guard(dev);
   check_status(lmcb_qk_norm_rope(
       query.data_ptr(), key.data_ptr(), to_lmcb_dtype(query.scalar_type()), token_stride(query),
@@ -895,7 +912,7 @@ void kv4_store(const torch::Tensor& key, const torch::Tensor& value, torch::Tens
 void kv4_load(const torch::Tensor& kv_cache, const torch::Tensor& slot_mapping, torch::Tensor& key,
               torch::Tensor& value) {
   check_kv4_rows(key, value, kv_cache, slot_mapping, "kv4_load");
-  TORCH_CHECK(!overlap(key, value), "kv4_load: key and value overlap");
+  TORCH_CHECK(!rows_overlap(key, value), "kv4_load: key and value overlap");
   const c10::cuda::CUDAGuard guard(kv_cache.device());
   check_status(lmcb_kv4_load(
       static_cast<const int32_t*>(kv_cache.data_ptr()), kv_cache.size(1), kv_cache.size(2),
@@ -933,7 +950,8 @@ void kv4_attention(const torch::Tensor& query, const torch::Tensor& kv_cache,
   } else {
     TORCH_CHECK(query.size(0) >= batch, who, ": without query_start every request has one query");
   }
-  TORCH_CHECK(!overlap(out, query) && !overlap(out, kv_cache), who, ": out overlaps an input");
+  TORCH_CHECK(!rows_overlap(out, query) && !overlap(out, kv_cache), who,
+              ": out overlaps an input");
   const c10::cuda::CUDAGuard guard(dev);
   size_t bytes = 0;
   check_status(lmcb_kv4_attention_workspace(batch, max_query_len, max_seq_len, num_kv_heads,

@@ -15,8 +15,8 @@
 // then taken as r_j / sv_j in the other sums too, so that a rounding of r_j
 // weighs v_j - o and not the code. The code c goes into the matrix instruction
 // as the fp16 bit pattern c, the subnormal c 2^-24, or shifted by four bits:
-// one AND makes two operands, with no conversion. The factors are kept in
-// range by powers of two that cancel: a query row is scaled to a largest
+// one AND makes two operands, with no conversion (see codes for fp16 results).
+// The factors are kept in range by powers of two that cancel: a query row is scaled to a largest
 // element of 2^13 ... 2^14 (bf16 queries become fp16 without loss, but for
 // elements below 2^-34 of the row's largest), and p_j sv_j by the largest sv
 // exponent seen so far.
@@ -39,8 +39,8 @@
 // requests are one line that is cut into equal pieces, so ragged lengths
 // leave no CTA idle; a second kernel joins requests that were cut.
 #include <climits>
-#include <cstdlib>
 #include <string>
+#include <type_traits>
 
 #include "kv4_attention.cuh"
 #include "kv4_plan.h"
@@ -130,7 +130,7 @@ __device__ __forceinline__ int32_t request_tiles(const AttnParams& p, const Requ
                                                  int32_t stage_tokens) {
   if (r.n == 0) return 0;
   const KeyRange k = request_range(p, r);
-  return k.count <= 0 ? 1 : (k.count + stage_tokens - 1) / stage_tokens;
+  return k.count <= 0 ? 1 : (k.count - 1) / stage_tokens + 1;
 }
 
 // Of a unit that several CTAs work on, [first, last] with x < y, and in z the
@@ -151,6 +151,25 @@ __device__ __forceinline__ int64_t active_ctas(int64_t total, int ctas) {
   return total < ctas ? total : ctas;
 }
 
+// Two codes of a cache word as operands: bits 0 ... 3 of both halves of x (kHigh
+// 0), or bits 4 ... 7, times 16 (kHigh 1).
+//
+// As they lie, c is the subnormal c 2^-24. That costs one AND, but the matrix
+// unit lines up what it adds by exponents, where a subnormal counts as 2^-14,
+// and cuts off 24 bits below: 2^-14 of a code. Results in bf16 do not show it.
+// fp16 results do (3.6e-4 of their size at 32000 tokens), so they take kNormal:
+// c on top of 1024, less 1024 and `zero`, exactly. V's zero is 8, the middle of
+// the codes, so that sums over a long cache stay near their result (2.1e-4).
+template <bool kNormal, int kHigh>
+__device__ __forceinline__ uint32_t codes(uint32_t x, int zero) {
+  const uint32_t bits = x & (kHigh ? 0x00f000f0u : 0x000f000fu);
+  if constexpr (!kNormal) return bits;
+  const __half2 base = __half2half2(__int2half_rn(1024 + (kHigh ? 16 : 1) * zero));
+  const uint32_t up = bits | 0x64006400u;
+  const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&up), base);
+  return *reinterpret_cast<const uint32_t*>(&c);
+}
+
 // Query operands of a unit: B fragments of q . k, and per column the factors
 //   s = acc * a * sk + zk * b  (log2 units).
 template <int D, int NT>
@@ -160,7 +179,13 @@ struct Query {
   int32_t pos[NT][2];  // position of the column's query token, -1: no such row
 };
 
-template <typename T, int D, int NT>
+// Codes of kNormal are counted in ones, else in 2^-24.
+template <bool kNormal>
+__host__ __device__ constexpr float code_unit() {
+  return kNormal ? 1.0f : 16777216.0f;
+}
+
+template <typename T, int D, int NT, bool kNormal>
 __device__ __forceinline__ void load_unit_query(const AttnParams& p, const Request& rq,
                                                 int kv_head, Query<D, NT>& q) {
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -210,7 +235,7 @@ __device__ __forceinline__ void load_unit_query(const AttnParams& p, const Reque
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int src = (2 * t + c) * 4;
-      q.a[n][c] = __shfl_sync(0xffffffffu, unit, src) * 16777216.0f;
+      q.a[n][c] = __shfl_sync(0xffffffffu, unit, src) * code_unit<kNormal>();
       q.b[n][c] = __shfl_sync(0xffffffffu, unit * sum, src);
       const int ps = tok < rq.n ? rq.len - rq.n + tok : -1;
       q.pos[n][c] = __shfl_sync(0xffffffffu, ps, src);
@@ -243,9 +268,12 @@ struct Running {
     vexp = 0;
   }
   // r = p sv 2^(29 - vexp), vexp the largest biased fp16 exponent of the sv so
-  // far: below 2^15 for p <= 1. acc counts codes of 2^-24.
+  // far: below 2^15 for p <= 1.
   __device__ __forceinline__ float value_factor() const { return pow2i(29 - vexp); }
-  __device__ __forceinline__ float value_unit() const { return pow2i(24 + vexp - 29); }
+  template <bool kNormal>
+  __device__ __forceinline__ float value_unit() const {
+    return pow2i(vexp - 29) * code_unit<kNormal>();
+  }
 };
 
 // Tokens are the rows of a score tile in the order sigma: its rows 2 i and
@@ -256,7 +284,7 @@ __device__ __forceinline__ int sigma(int i) { return i % 2 ? ((i / 2 + 2) & 3) +
 
 // ST * 16 tokens of a stage, the warp's turn of them. kAll: every token is
 // there and seen by every query row.
-template <int D, int NT, int ST, bool kAll>
+template <int D, int NT, int ST, bool kAll, bool kNormal>
 __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* stage,
                                           const uint32_t* valid, int first, int code_off,
                                           int par_off, const KeyRange& range, int32_t v0,
@@ -299,10 +327,11 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t x0 = kw[0][w] >> (8 * j), x1 = kw[1][w] >> (8 * j);
+        const uint32_t a0 = codes<kNormal, 0>(x0, 0), a1 = codes<kNormal, 0>(x1, 0);
+        const uint32_t a2 = codes<kNormal, 1>(x0, 0), a3 = codes<kNormal, 1>(x1, 0);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16(s[u][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u,
-                  q.frag[n][2 * w + j][0], q.frag[n][2 * w + j][1]);
+          mma_f16(s[u][n], a0, a1, a2, a3, q.frag[n][2 * w + j][0], q.frag[n][2 * w + j][1]);
         }
       }
     }
@@ -371,6 +400,7 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
     for (int i = 0; i < 2; ++i) {
       sf[i] = half_lo(vpar[u][i]) * vfac;
       zv[i] = half_hi(vpar[u][i]);
+      if constexpr (kNormal) zv[i] = fmaf(8.0f, half_lo(vpar[u][i]), zv[i]);
       // r is a normal fp16 number for p down to 2^-14 only where sf >= 1;
       // below, its rounding says nothing about p
       back[i] = sf[i] >= 1.0f ? rcp_approx(sf[i]) : 0.0f;
@@ -413,10 +443,11 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
       for (int i = 0; i < 4; ++i) {
         const uint32_t x0 = (i < 2 ? lo0 : hi0) >> (8 * (i & 1));
         const uint32_t x1 = (i < 2 ? lo1 : hi1) >> (8 * (i & 1));
+        const uint32_t a0 = codes<kNormal, 0>(x0, 8), a1 = codes<kNormal, 1>(x0, 8);
+        const uint32_t a2 = codes<kNormal, 0>(x1, 8), a3 = codes<kNormal, 1>(x1, 8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16(st.acc[4 * w + i][n], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu,
-                  x1 & 0x00f000f0u, pf[n][0], pf[n][1]);
+          mma_f16(st.acc[4 * w + i][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
         }
       }
     }
@@ -452,7 +483,8 @@ __device__ __forceinline__ void write_rows(const DecodeParams& p, const Request&
                                            int head, int slot, const Running<D, NT>& st) {
   constexpr int N = D / 8;
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const float unit = st.value_unit(), unit16 = unit * 0.0625f;
+  const float unit = st.template value_unit<std::is_same<T, __half>::value>();
+  const float unit16 = unit * 0.0625f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -506,7 +538,8 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
       for (int c = 0; c < 2; ++c) s_m[(turn * heads + head) * R + n * 8 + 2 * t + c] = st.m[n][c];
   }
   __syncthreads();
-  const float unit = st.value_unit(), unit16 = unit * 0.0625f;
+  const float unit = st.template value_unit<std::is_same<T, __half>::value>();
+  const float unit16 = unit * 0.0625f;
   float f[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -682,6 +715,7 @@ __device__ __forceinline__ bool run_line(const DecodeParams& p, const Line& line
   const int head = warp % p.heads, turn = warp / p.heads;
   const int first = turn * ST * 16;  // this warp's tokens of a stage
   const uint32_t count = static_cast<uint32_t>(line.end - line.begin);
+  constexpr bool kNormal = std::is_same<T, __half>::value;
   bool ok = true;
   if (warp < p.stages && static_cast<uint32_t>(warp) < count) {
     produce(p, line, warp, data, ring, D / 2);
@@ -710,7 +744,7 @@ __device__ __forceinline__ bool run_line(const DecodeParams& p, const Line& line
                             ? a.kv_heads * (D / 2) + head * 4
                             : p.heads * (D / 2) +
                                   ((a.kv_heads * (D / 2) + group * p.heads * 4) & 15) + head * 4;
-    if (working) load_unit_query<T, D, NT>(a, rq, kv_head, q);
+    if (working) load_unit_query<T, D, NT, kNormal>(a, rq, kv_head, q);
     st.reset();
     for (const uint32_t j_end = j + steps; j < j_end; ++j, ++t) {
       if (j > 0 && j % kWarps == static_cast<uint32_t>(warp) && j - 1 + p.stages < count && ok) {
@@ -726,10 +760,10 @@ __device__ __forceinline__ bool run_line(const DecodeParams& p, const Line& line
           all = all && ((ring.valid[stage][tok / 32] >> (tok % 32)) & 0xffffu) == 0xffffu;
         }
         if (all) {
-          take_tile<D, NT, ST, true>(p, at, ring.valid[stage], first, code_off, par_off, range,
+          take_tile<D, NT, ST, true, kNormal>(p, at, ring.valid[stage], first, code_off, par_off, range,
                                      t * p.stage_tokens, false, q, st);
         } else {
-          take_tile<D, NT, ST, false>(p, at, ring.valid[stage], first, code_off, par_off, range,
+          take_tile<D, NT, ST, false, kNormal>(p, at, ring.valid[stage], first, code_off, par_off, range,
                                       t * p.stage_tokens, mask, q, st);
         }
       }
@@ -1021,6 +1055,7 @@ cudaError_t launch_size(const DecodeParams& p, const Plan& pl, int64_t head_size
 bool is_decode(int64_t max_query, int64_t group) { return max_query * group <= 16; }
 
 constexpr int64_t kMaxBatch = 4096;  // tiles before each request, in shared memory
+constexpr int64_t kMaxKeys = INT_MAX - 1024;  // of a table row: a tile's end is an int32
 
 int check_shape(const std::string& who, int64_t batch, int64_t max_query, int64_t max_len,
                 int64_t kv_heads, int64_t query_heads, int64_t head_size, int64_t window,
@@ -1090,10 +1125,14 @@ int lmcb_kv4_attention(const void* query, int type, int64_t queryTokenStride, in
   if (st != LMCB_OK) return st;
   if (numQueryRows < 0 || numQueryRows > INT_MAX / 2 || numBlocks < 0 || blockSize <= 0 ||
       (numBlocks > 0 && blockSize > INT_MAX / numBlocks) || tableCols < 0 ||
-      tableStride < tableCols || (tableCols > 0 && blockSize > INT_MAX / tableCols) ||
+      tableStride < tableCols || (tableCols > 0 && blockSize > kv4::kMaxKeys / tableCols) ||
       queryTokenStride < numQueryHeads * headSize || outTokenStride < numQueryHeads * headSize ||
       (queryStart == nullptr && (maxQueryLen < 1 || numQueryRows < batch))) {
     return fail(LMCB_ERR_INVALID_ARGUMENT, who + ": invalid shape.");
+  }
+  // tiles of 16 keys of all requests are counted in an int32
+  if (batch > 0 && (tableCols * blockSize + 15) / 16 > INT_MAX / batch) {
+    return fail(LMCB_ERR_CAPACITY, who + ": too many keys in one call.");
   }
   if (batch == 0 || numQueryRows == 0 || maxQueryLen == 0) return LMCB_OK;
   if (query == nullptr || out == nullptr || seqLens == nullptr ||

@@ -1,11 +1,11 @@
 // kv4_cache.cu -- rows into and out of the paged KV cache held in 4 bits
 // (kv4_store, kv4_load; layout in kv4.cuh).
 //
-// A head row x of D values keeps z = fp16(min x), s = fp16((max x - min x) /
-// 15) and the codes clamp(rne((x - z) / s), 0, 15); it reads back as z + s c.
-// Minimum, difference and quotient are fp32, each rounded once; s and z are
-// fp16 because an attention kernel multiplies by them in fp32 anyway and a
-// row's 4 bytes are then 1/17 of its 68 (D = 128). NaN counts as 0 and values
+// A head row x of D values keeps z = fp16(min x), s = fp16((max x - min x) r),
+// r the fp32 number nearest to 1 / 15, and the codes clamp(rne((x - z) / s), 0,
+// 15); it reads back as z + s c. Difference and product are fp32, each rounded
+// once; s and z are fp16 because an attention kernel multiplies by them in fp32
+// anyway and a row's 4 bytes are then 1/17 of its 68 (D = 128). NaN counts as 0 and values
 // beyond the fp16 range as its ends, so that every row is finite.
 //
 // The code is the exact one, see word_of: it depends on no rounding of a
@@ -294,11 +294,7 @@ __device__ __forceinline__ void store_rows(const Eight<T> (&x)[kHeads], float (&
         hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
       }
     }
-    // The fp32 quotient by 15, rounded once: that of 24 bits by 15 is never closer
-    // than 2^-29 of itself to a border between two fp32 numbers, and the product
-    // in 64 bits is off by 2^-52.
-    const float span = static_cast<float>(static_cast<double>(hi[k] - lo[k]) * (1.0 / 15.0));
-    const __half sh = __float2half_rn(span);
+    const __half sh = __float2half_rn(__fmul_rn(hi[k] - lo[k], 1.0f / 15.0f));
     // + 0: a zero of either sign is kept as +0, so equal rows have equal words
     const float z = __half2float(__float2half_rn(lo[k])) + 0.0f;
     const float s = __half2float(sh);

@@ -277,7 +277,7 @@ struct Control {
   float4 kpar[kMaxStages][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
   uint32_t valid[kMaxStages][4];      // two bits a token, 16 tokens each
   float2 vexp[kMaxStages][4];         // e of 16 tokens, twice
-  float2 row[2 * kRows];              // a, sum of q 2^-24; at the end m, l
+  float2 row[2 * kRows];              // a, sum of q in its unit; at the end m, l
   float e[2 * kRows];                 // at the end
   uint32_t tmem;
 };
@@ -328,9 +328,11 @@ __device__ __forceinline__ void load_row(const AttnParams& p, const Request& rq,
     }
     *reinterpret_cast<uint4*>(smem + (i / 8) * L::kQPanel + swizzled(r, i % 8)) = out;
   }
-  // a is never zero, so that a key that is not seen stays at -inf
-  factors = make_float2(fmaxf(fabsf(p.scale_log2) * pow2i(e - 13) * 16777216.0f, 1.2e-38f),
-                        sum * 5.9604645e-8f);
+  // codes count 2^-24, or 1 (expand_k); a is never zero, so that a key that is
+  // not seen stays at -inf
+  constexpr float kUnit = std::is_same<T, __half>::value ? 1.0f : 16777216.0f;
+  factors = make_float2(fmaxf(fabsf(p.scale_log2) * pow2i(e - 13) * kUnit, 1.2e-38f),
+                        sum / kUnit);
 }
 
 // ---------------------------------------------------------------------------
@@ -400,12 +402,21 @@ __device__ __forceinline__ uint4 expand_v(uint32_t w, __half2 s24, __half2 s20, 
                     half2_bits(__hfma2(as_half2(x & 0x00f000f0u), s20, z)));
 }
 
+// fp16 results take normal numbers, c and 16 c on top of 1024 less 1024: the
+// matrix unit cuts off bits of sums of subnormals (codes in the decode kernel).
+template <bool kNormal>
 __device__ __forceinline__ uint4 expand_k(uint32_t w) {
   const uint32_t x = w >> 8;
-  return make_uint4(w & 0x000f000fu, w & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u);
+  uint32_t r[4] = {w & 0x000f000fu, w & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u};
+  if constexpr (kNormal) {
+    const __half2 base = __half2half2(__ushort_as_half(0x6400));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = half2_bits(__hsub2(as_half2(r[j] | 0x64006400u), base));
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <int D>
+template <int D, bool kNormal>
 __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range, int b,
                                       int kv_head, int32_t t0, int32_t tiles, uint8_t* smem,
                                       Control& ctl) {
@@ -469,7 +480,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint8_t* to = k + n * L::kPanel + swizzled(tok, piece + j);
-        *reinterpret_cast<uint4*>(to) = expand_k(kw[j]);
+        *reinterpret_cast<uint4*>(to) = expand_k<kNormal>(kw[j]);
         *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], s24, s20, z2);
       }
     }
@@ -911,7 +922,7 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
     }
   } else if (warp >= L::kBring) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    ok = bring<D>(a, range, b, kv_head, t0, t1 - t0, smem + L::kUnits * L::kQ, ctl);
+    ok = bring<D, kTwo>(a, range, b, kv_head, t0, t1 - t0, smem + L::kUnits * L::kQ, ctl);
   } else if (warp < 8 * units) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     ok = attend<D, kTwo>(a, range, t0, t1 - t0, pos_first, pos_last, rq, first_row, ctl);

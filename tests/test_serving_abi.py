@@ -131,6 +131,7 @@ def attn_args(**kw):
     (dict(blocks=1 << 28), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(cols=1 << 28, ts=1 << 28), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(batch=4097, rows=4097), abi.LMCB_ERR_CAPACITY),
+    (dict(batch=4096, rows=4096, cols=1 << 20, ts=1 << 20), abi.LMCB_ERR_CAPACITY),
     (dict(q=None), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(lens=None), abi.LMCB_ERR_INVALID_ARGUMENT),
     (dict(cache=P + 4), abi.LMCB_ERR_INVALID_ARGUMENT),

@@ -328,6 +328,18 @@ def test_qk_refusals():
     a[9] = qo[:, :1]
     with pytest.raises(RuntimeError, match="overlap"):
         c_ops.qk_norm_rope(*a)
+    for queries, keys in ((q, q), (both[:4], both[1:])):  # in place over each other
+        a = list(ok)
+        a[0] = a[8] = queries
+        a[1] = a[9] = keys
+        with pytest.raises(RuntimeError, match="overlap"):
+            c_ops.qk_norm_rope(*a)
+    # parts of one packed output are no overlap
+    packed = torch.zeros(4, 3 * 64, device=DEV)
+    a = list(ok)
+    a[8], a[9] = packed[:, :128].view(4, 2, 64), packed[:, 128:].view(4, 1, 64)
+    c_ops.qk_norm_rope(*a)
+    assert torch.equal(a[8], qo) and torch.equal(a[9], ko)
 
 
 # ---------------------------------------------------------------------------
@@ -490,6 +502,10 @@ def test_kv4_out_of_range_slots_and_refusals():
     bad("dense", key=x.transpose(0, 1), value=x.transpose(0, 1))
     with pytest.raises(RuntimeError, match="overlap"):
         c_ops.kv4_load(cache, slots, out, out)
+    packed = torch.full((4, 4 * 64), 9.0, device=DEV)  # key and value side by side
+    c_ops.kv4_load(cache, slots, packed[:, :128].view(4, 2, 64), packed[:, 128:].view(4, 2, 64))
+    assert torch.equal(packed[0, :128].view(2, 64), packed[0, 128:].view(2, 64))
+    assert bool((packed[1:] == 9).all())
     c_ops.kv4_store(x[:0], x[:0], cache, slots[:0])
 
 
@@ -812,6 +828,37 @@ def test_attention_refusals():
     a[0], a[11] = b.q.float(), out.float()
     with pytest.raises(RuntimeError, match="bf16 or fp16"):
         c_ops.kv4_attention(*a)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 3.0])
+@pytest.mark.parametrize("qlens", [[1, 1], [30, 2]])
+def test_attention_other_scales(scale, qlens):
+    """No scale (the mean of the values), a negative and a large one."""
+    for d, dtype in ((128, torch.bfloat16), (64, torch.float16)):
+        b = Batch([300, 77], qlens, 2, 4, d, 16, dtype, seed=d)
+        b.scale = scale
+        b.check(b.run())
+        b.check(b.run(20, 3), 20, 3)
+
+
+def test_attention_shared_pages():
+    """Two requests on the same pages (a shared prefix) give the same rows."""
+    b = Batch([333, 333, 90], [1, 1, 1], 2, 4, 128, 16, torch.bfloat16)
+    b.table[1] = b.table[0]
+    b.q[1] = b.q[0]
+    out = b.run()
+    assert torch.equal(out[0], out[1])
+
+
+def test_attention_into_a_packed_buffer():
+    """out beside the queries in one buffer of rows."""
+    b = Batch([50, 70], [1, 1], 2, 4, 64, 16, torch.float16)
+    want = b.run()
+    buf = torch.zeros(2, 16 * 64, dtype=torch.float16, device=DEV)
+    q, out = buf[:, : 8 * 64].view(2, 8, 64), buf[:, 8 * 64 :].view(2, 8, 64)
+    q.copy_(b.q)
+    b.run(q=q, out=out)
+    assert torch.equal(out, want) and torch.equal(q, b.q)
 
 
 # ---------------------------------------------------------------------------
