@@ -21,6 +21,7 @@
 
 #include <climits>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv4.cuh"
@@ -72,6 +73,22 @@ template <typename T>
 struct alignas(16) Eight {
   T v[8];
 };
+
+// Eight elements as floats; bf16 are the high halves of theirs.
+template <typename T>
+__device__ __forceinline__ void floats_of(const Eight<T>& x, float (&v)[8]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(x.v[i]);
+  }
+}
 
 template <typename T, bool kVec>
 __device__ __forceinline__ Eight<T> load8(const T* src) {
@@ -161,8 +178,8 @@ __device__ __forceinline__ void row_range(const Eight<T>& x, bool active, float&
 // 2^-22 <= (2 |z| / s / 15 + 1) 2^-22, so 15 y by (|z| / s + 8) 2^-21. Adding
 // 1.5 2^23 rounds 15 y to an integer, ties to even, in the sum's low bits; a
 // multiply-add by 16^i puts it in its place, and what the eight exponent fields
-// add up to is one constant. Only an element that lies that close to the border
-// between two codes is taken again, in 64 bits: three in a hundred thousand.
+// add up to is one constant. Only a word with an element that lies that close to
+// the border between two codes is taken again, in 64 bits.
 struct Coder {
   float inv, shift, sure;  // 1 / (15 s), -z / (15 s), and how close is too close
 
@@ -175,60 +192,50 @@ struct Coder {
 
 constexpr float kMagic = 12582912.0f;
 
-// Two fp32 values an instruction.
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // `off` grows to how far the word's elements are from their codes, in steps.
 __device__ __forceinline__ uint32_t word_of(const float (&v)[8], const Coder& c, float& off) {
   constexpr uint32_t kBias = 0x4B400000u * 0x11111111u;
-  const uint64_t magic = pack2(kMagic, kMagic), fifteen = pack2(15.0f, 15.0f);
-  const uint64_t minus = pack2(-1.0f, -1.0f);
   uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const uint64_t y = pack2(__saturatef(fmaf(v[i], c.inv, c.shift)),
-                             __saturatef(fmaf(v[i + 1], c.inv, c.shift)));
-    const uint64_t r = fma2(y, fifteen, magic);
-    const float2 away = unpack2(fma2(y, fifteen, fma2(r, minus, magic)));
-    off = fmaxf(off, fmaxf(fabsf(away.x), fabsf(away.y)));
-    const float2 bits = unpack2(r);
-    word += __float_as_uint(bits.x) << (4 * i);
-    word += __float_as_uint(bits.y) << (4 * i + 4);
+  for (int i = 0; i < 8; ++i) {
+    const float y = __saturatef(fmaf(v[i], c.inv, c.shift));
+    const float r = fmaf(y, 15.0f, kMagic);
+    off = fmaxf(off, fabsf(fmaf(y, 15.0f, kMagic - r)));
+    word += __float_as_uint(r) << (4 * i);
   }
   return word - kBias;
 }
 
-// The word again, with the elements that are too close to a border in 64 bits.
-__device__ __noinline__ uint32_t exact_word(float v0, float v1, float v2, float v3, float v4,
-                                            float v5, float v6, float v7, uint32_t word, float z,
-                                            float s) {
-  const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+// z and s of a head row whose values are in [lo, hi].
+__device__ __forceinline__ void row_params(float lo, float hi, float& z, float& s) {
+  s = __half2float(__float2half_rn(__fmul_rn(hi - lo, 1.0f / 15.0f)));
+  // + 0: a zero of either sign is kept as +0, so equal rows have equal words
+  z = __half2float(__float2half_rn(lo)) + 0.0f;
+}
+
+// The elements of a word that are too close to a border, again, from global
+// memory: x - z, in 64 bits, against the border (k + 1/2) s, which is exact in
+// fp32. Out of line and apart from the rest, so that the common path keeps its
+// registers.
+template <typename T>
+__device__ __noinline__ void exact_word(const T* src, float z, float s, int32_t* dst) {
   const Coder c(z, s);
+  uint32_t word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = __saturatef(fmaf(v[i], c.inv, c.shift));
-    if (fabsf(fmaf(y, 15.0f, kMagic - fmaf(y, 15.0f, kMagic))) >= c.sure) {
-      const double q =
-          (static_cast<double>(v[i]) - static_cast<double>(z)) / static_cast<double>(s);
-      const uint32_t code = static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
-      word = (word & ~(15u << (4 * i))) | (code << (4 * i));
+    const float x = finite_half_range(to_float(src[i]));
+    const float q = __saturatef(fmaf(x, c.inv, c.shift)) * 15.0f;
+    uint32_t code = static_cast<uint32_t>(q + 0.5f);
+    if (fabsf(q - rintf(q)) >= c.sure) {
+      const float low = floorf(q);
+      const double d = static_cast<double>(x) - static_cast<double>(z);
+      const double border = static_cast<double>((low + 0.5f) * s);
+      const uint32_t k = static_cast<uint32_t>(low);
+      code = d > border ? k + 1 : (d < border ? k : (k + 1) & ~1u);
     }
+    word |= code << (4 * i);
   }
-  return word;
+  *dst = static_cast<int32_t>(word);
 }
 
 __device__ __forceinline__ int64_t slot_of(const Kv4Params& p, uint32_t token) {
@@ -251,7 +258,9 @@ struct Item {
 template <int kHeads>
 __device__ __forceinline__ Item item_of(const Kv4Params& p, uint64_t at, bool flag) {
   Item it;
-  it.count = 0;
+  it.half = it.count = 0;
+  it.token = it.head = 0;
+  it.slot = -1;
   if (at >= 2ull * p.items_per_half) return it;
   it.half = at >= p.items_per_half;
   const uint32_t in_half = static_cast<uint32_t>(at) - (it.half ? p.items_per_half : 0);
@@ -267,16 +276,18 @@ __device__ __forceinline__ Item item_of(const Kv4Params& p, uint64_t at, bool fl
 }
 
 // The head rows x of a group into the cache. kWild: some row of the warp holds
-// NaN or a value beyond the fp16 range.
+// NaN or a value beyond the fp16 range. Returns a bit for each row whose word
+// of this lane has an element too close to a border.
 template <typename T, int kGroup, int kHeads, bool kFull, bool kWild>
-__device__ __forceinline__ void store_rows(const Eight<T> (&x)[kHeads], float (&lo)[kHeads],
-                                           float (&hi)[kHeads], bool active, int count, int lane,
-                                           int words, int32_t* codes, int32_t* params) {
+__device__ __forceinline__ uint32_t store_rows(const Eight<T> (&x)[kHeads], float (&lo)[kHeads],
+                                               float (&hi)[kHeads], bool active, int count,
+                                               int lane, int words, int32_t* codes,
+                                               int32_t* params) {
+  uint32_t close = 0;
 #pragma unroll
   for (int k = 0; k < kHeads; ++k) {
     float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(x[k].v[i]);
+    floats_of(x[k], v);
     if constexpr (kWild) {
       lo[k] = INFINITY;
       hi[k] = -INFINITY;
@@ -294,24 +305,23 @@ __device__ __forceinline__ void store_rows(const Eight<T> (&x)[kHeads], float (&
         hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
       }
     }
-    const __half sh = __float2half_rn(__fmul_rn(hi[k] - lo[k], 1.0f / 15.0f));
-    // + 0: a zero of either sign is kept as +0, so equal rows have equal words
-    const float z = __half2float(__float2half_rn(lo[k])) + 0.0f;
-    const float s = __half2float(sh);
+    float z, s;
+    row_params(lo[k], hi[k], z, s);
     const Coder c(z, s);
     float off = 0.0f;
     uint32_t word = word_of(v, c, off);
-    if (off >= c.sure) word = exact_word(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], word, z, s);
     if (s == 0.0f) word = 0;  // one value only: z
     if ((kFull ? count > 0 : k < count) && active) {
       codes[k * words] = static_cast<int32_t>(word);
+      if (s > 0.0f && off >= c.sure) close |= 1u << k;
       if (lane == 0) {
         params[k] = static_cast<int32_t>(
-            static_cast<uint32_t>(__half_as_ushort(sh)) |
+            static_cast<uint32_t>(__half_as_ushort(__float2half_rn(s))) |
             (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(z))) << 16));
       }
     }
   }
+  return close;
 }
 
 // kGroup lanes share a head row (D <= 8 * kGroup).
@@ -327,11 +337,11 @@ kv4_store_kernel(const __grid_constant__ Kv4Params p) {
        base += static_cast<uint64_t>(gridDim.x) * kGroups) {
     const Item it = item_of<kHeads>(p, base + threadIdx.x / kGroup, lane == 0);
     Eight<T> x[kHeads] = {};
+    const T* src = static_cast<const T*>(it.half ? p.src[1] : p.src[0]) +
+                   static_cast<int64_t>(it.token) *
+                       (it.half ? p.token_stride[1] : p.token_stride[0]) +
+                   static_cast<int64_t>(it.head) * D + lane * 8;
     if (it.count > 0 && active) {
-      const T* src = static_cast<const T*>(it.half ? p.src[1] : p.src[0]) +
-                     static_cast<int64_t>(it.token) *
-                         (it.half ? p.token_stride[1] : p.token_stride[0]) +
-                     static_cast<int64_t>(it.head) * D + lane * 8;
 #pragma unroll
       for (int k = 0; k < kHeads; ++k) {
         if (kFull || k < it.count) x[k] = load8<T, kVec>(src + k * D);
@@ -347,12 +357,21 @@ kv4_store_kernel(const __grid_constant__ Kv4Params p) {
       row_range<T, kGroup>(x[k], active, lo[k], hi[k]);
       tame = tame && lo[k] >= -65504.0f && hi[k] <= 65504.0f;
     }
+    uint32_t close;
     if (__all_sync(0xffffffffu, tame)) {
-      store_rows<T, kGroup, kHeads, kFull, false>(x, lo, hi, active, it.count, lane, D / 8, codes,
-                                                  params);
+      close = store_rows<T, kGroup, kHeads, kFull, false>(x, lo, hi, active, it.count, lane, D / 8,
+                                                          codes, params);
     } else {
-      store_rows<T, kGroup, kHeads, kFull, true>(x, lo, hi, active, it.count, lane, D / 8, codes,
-                                                 params);
+      close = store_rows<T, kGroup, kHeads, kFull, true>(x, lo, hi, active, it.count, lane, D / 8,
+                                                         codes, params);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      if (close & (1u << k)) {
+        float z, s;
+        row_params(lo[k], hi[k], z, s);
+        exact_word<T>(src + k * D, z, s, codes + k * (D / 8));
+      }
     }
   }
 }
