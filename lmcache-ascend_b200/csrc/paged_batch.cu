@@ -12,6 +12,12 @@
 // writing; the thread that has a new page's first token writes it there. What is
 // left is one search over the prefix sums for each group of consecutive tokens
 // and the writes of slots and positions.
+//
+// Measured: 1021 requests with 765,000 tokens 14.0 us, where writing and reading
+// the 12.9 MB takes 2.0: about 5 us are the launch, the rest is a chain of the
+// length loads, two scans and the first search that every CTA goes through before
+// its first store. 8 requests with a token each 6.4 us, which is the call itself
+// (256 threads there; 1024 cost 2 us more, and nothing from 96 requests on).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -24,7 +30,7 @@
 namespace lmcb {
 namespace {
 
-constexpr int kBatchThreads = 1024;  // 256 for a batch that they cover
+constexpr int kBatchThreads = 1024;  // 256 where they cover requests and tokens
 constexpr int kBatchMaxRequests = 16384;  // 12 bytes of shared memory each
 constexpr int kTokensPerThread = 4;
 
