@@ -462,21 +462,12 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
   }
 }
 
-// Warps that share a head add up in shared memory. Up to 128 values a row and 8
-// rows each has a place of its own there (32 KB), and all threads add them;
-// larger ones share a place, in turn.
-template <int D, int NT>
-__host__ __device__ constexpr bool own_places() {
-  return D * NT <= 128;
-}
-
-template <int D, int NT>
-__host__ __device__ constexpr size_t merge_bytes(int heads) {
-  // one warp a head: nothing to merge
-  return kWarps / heads == 1
-             ? 0
-             : ((own_places<D, NT>() ? kWarps : static_cast<size_t>(heads)) * 8 * NT * (D + 1) +
-                kWarps * 8 * NT) * 4;
+// Warps that share a head have a place each in shared memory, and all threads
+// add them up: bytes for 8 * nt rows (66 KB at most; one warp a head: nothing to
+// merge). Adding to one place in turn took less room and more time: 34.8 us
+// against 20.5 for one request of 512 tokens, one KV head of 256.
+__host__ __device__ constexpr int64_t merge_bytes(int heads, int nt, int64_t head_size) {
+  return kWarps / heads == 1 ? 0 : kWarps * 8 * nt * (head_size + 2) * 4;
 }
 
 // Where a query row's output, or this CTA's part of it, goes.
@@ -530,12 +521,11 @@ template <typename T, int D, int NT>
 __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request& rq, int group,
                                            int slot, const Running<D, NT>& st, float* smem) {
   constexpr int R = 8 * NT;
-  constexpr bool kOwn = own_places<D, NT>();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int heads = p.heads, turns = p.turns;
   const int head = warp % heads, turn = warp / heads;
   const bool working = turn < turns;
-  const int places = kOwn ? turns * heads : heads;
+  const int places = turns * heads, place = turn * heads + head;
   float* s_o = smem;                   // [places][R][D]
   float* s_l = s_o + places * R * D;   // [places][R]
   float* s_m = s_l + places * R;       // [turns][heads][R]
@@ -557,38 +547,24 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
       for (int w = 0; w < turns; ++w) m = fmaxf(m, s_m[(w * heads + head) * R + n * 8 + 2 * t + c]);
       f[n][c] = m == -INFINITY ? 0.0f : exp2_approx(st.m[n][c] - m);
     }
-  for (int w = 0; w < (kOwn ? 1 : turns); ++w) {
-    if (kOwn ? working : w == turn) {
-      const int place = kOwn ? turn * heads + head : head;
-      const bool add = !kOwn && w > 0;
+  if (working) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = n * 8 + 2 * t + c;
-          if (col >= p.rows) continue;
-          float* o = s_o + (place * R + col) * D + g * (D / 8);
+      for (int c = 0; c < 2; ++c) {
+        const int col = n * 8 + 2 * t + c;
+        if (col >= p.rows) continue;
+        float* o = s_o + (place * R + col) * D + g * (D / 8);
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            float2 v;
-            v.x = fmaf(st.acc[i][n][c], unit, st.z[n][c]) * f[n][c];
-            v.y = fmaf(st.acc[i][n][c + 2], unit16, st.z[n][c]) * f[n][c];
-            float2* at = reinterpret_cast<float2*>(o + 2 * i);
-            if (add) {
-              const float2 old = *at;
-              v.x += old.x;
-              v.y += old.y;
-            }
-            *at = v;
-          }
-          if (g == 0) {
-            const float l = st.l[n][c] * f[n][c];
-            s_l[place * R + col] = add ? s_l[place * R + col] + l : l;
-          }
+        for (int i = 0; i < D / 16; ++i) {
+          *reinterpret_cast<float2*>(o + 2 * i) =
+              make_float2(fmaf(st.acc[i][n][c], unit, st.z[n][c]) * f[n][c],
+                          fmaf(st.acc[i][n][c + 2], unit16, st.z[n][c]) * f[n][c]);
         }
-    }
-    __syncthreads();
+        if (g == 0) s_l[place * R + col] = st.l[n][c] * f[n][c];
+      }
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < heads * p.rows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), e = (i % (D / 4)) * 4;
     const int h = row / p.rows, col = row % p.rows;
@@ -597,14 +573,14 @@ __device__ __forceinline__ void merge_rows(const DecodeParams& p, const Request&
     if (tok >= rq.n || kv_head >= p.a.kv_heads) continue;
     float4 v = *reinterpret_cast<const float4*>(s_o + (h * R + col) * D + e);
     float l = s_l[h * R + col];
-    for (int w = 1; w < (kOwn ? turns : 1); ++w) {
-      const int place = w * heads + h;
-      const float4 u = *reinterpret_cast<const float4*>(s_o + (place * R + col) * D + e);
+    for (int w = 1; w < turns; ++w) {
+      const int other = w * heads + h;
+      const float4 u = *reinterpret_cast<const float4*>(s_o + (other * R + col) * D + e);
       v.x += u.x;
       v.y += u.y;
       v.z += u.z;
       v.w += u.w;
-      l += s_l[place * R + col];
+      l += s_l[other * R + col];
     }
     if (slot < 0) {
       const float inv = inverse_sum(l);
@@ -813,7 +789,7 @@ kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ int32_t s_warp[kWarps];
   float* merge = reinterpret_cast<float*>(decode_smem + p.stages * p.stage_bytes);
   int32_t* prefix = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(merge) +
-                                               merge_bytes<D, NT>(p.heads));
+                                               merge_bytes(p.heads, NT, D));
   const AttnParams& a = p.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   pdl_launch_dependents();  // the joining kernel may take its place; it waits for this one
@@ -991,10 +967,7 @@ Plan make_plan(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_hea
                      : pl.heads * (head_size / 2) + (pl.heads * 4 + 12 + 15) / 16 * 16);
   pl.stage_bytes = 2 * pl.stage_tokens * pl.tok_stride;
   const int per_sm = head_size * pl.nt <= 128 ? 2 : 1;
-  const int64_t merge =
-      pl.turns == 1 ? 0
-                    : ((head_size * pl.nt <= 128 ? kWarps : pl.heads) * 8 * pl.nt * (head_size + 1) +
-                       kWarps * 8 * pl.nt) * 4;
+  const int64_t merge = merge_bytes(pl.heads, pl.nt, head_size);
   const int64_t room = 220 * 1024 / per_sm - merge - (batch + 1) * 4 - 1024;
   pl.stages = static_cast<int>(room / pl.stage_bytes);
   if (pl.stages > kMaxStages) pl.stages = kMaxStages;
@@ -1012,7 +985,7 @@ Plan make_plan(int64_t batch, int64_t max_query, int64_t max_len, int64_t kv_hea
 
 template <typename T, int D, int NT, int ST>
 cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(p.stages) * p.stage_bytes + merge_bytes<D, NT>(p.heads) +
+  const size_t smem = static_cast<size_t>(p.stages) * p.stage_bytes + merge_bytes(p.heads, NT, D) +
                       (static_cast<size_t>(p.a.batch) + 1) * 4;
   // 47 KB: the static shared memory counts towards the 48 KB that need no limit
   cudaError_t err = ensure_smem_limit<kv4_decode_kernel<T, D, NT, ST>>(
@@ -1062,10 +1035,10 @@ cudaError_t launch_size(const DecodeParams& p, const Plan& pl, int64_t head_size
 // The decode kernel takes up to 16 query rows a KV head, and with heads of 256,
 // whose second eight rows leave it too few registers, up to 8. The time of the
 // other kernel hardly depends on the rows up to 128. Measured, decode / rows: 64
-// requests of 8192 tokens, 8 KV heads of 128: 8 rows 152 / 612 us, 16 rows 320
-// ... 354 / 616; one request of 32768, one head: 16 rows 39 / 59. Heads of 256, 64
-// requests of 8192, 2 KV heads: 8 rows 131 / 244, 16 rows 276 / 246; 4 requests of
-// 4096: 31 / 35 and 47 / 35; with 8 KV heads 16 rows cost 227 / 248.
+// requests of 8192 tokens, 8 KV heads of 128: 8 rows 150 / 612 us, 16 rows 317
+// ... 354 / 616; one request of 32768, one head: 16 rows 37 / 59. Heads of 256, 64
+// requests of 8192, 2 KV heads: 8 rows 117 / 244, 16 rows 262 / 244; 4 requests of
+// 4096: 25 / 35 and 41 / 35; 16 of 8192 with 8 KV heads: 100 / 246 and 242 / 246.
 bool is_decode(int64_t max_query, int64_t group, int64_t head_size) {
   return max_query * group <= (head_size > 128 ? 8 : 16);
 }
