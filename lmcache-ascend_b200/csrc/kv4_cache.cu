@@ -16,7 +16,7 @@
 // 16-byte access of a 16-bit type), and a lane has up to kMost rows in flight.
 //
 // Measured, 40001 tokens of 8 heads of 128 in bf16 (208 MB each way): load 37 us,
-// 5.6 TB/s, bound by memory; store 71.6 us, 2.9 TB/s, bound by issue slots (75%
+// 5.6 TB/s, bound by memory; store 72 us, 2.9 TB/s, bound by issue slots (75%
 // of them used: 174 instructions a warp for two head rows, of which half find the
 // codes and the sixth part the row's minimum and maximum). With a division per
 // element instead of the corrected product it took 215 us.
@@ -219,10 +219,12 @@ __device__ __forceinline__ void row_params(float lo, float hi, float& z, float& 
   z = __half2float(__float2half_rn(lo)) + 0.0f;
 }
 
-// The elements of a word that are too close to a border, again, from global
-// memory: x - z, in 64 bits, against the border (k + 1/2) s, which is exact in
-// fp32. Out of line and apart from the rest, so that the common path keeps its
-// registers.
+// A word with elements too close to a border, again, from global memory: their x - z,
+// in 64 bits, against a border (k + 1/2) s, which is exact in fp32. k is the
+// quotient's floor, or off by one only where the quotient is within an fp32
+// rounding of a whole number and both its borders are far. It is at most 14: a
+// row that is narrow against its offset has quotients far beyond 15. Out of line
+// and apart from the rest, so that the common path keeps its registers.
 template <typename T>
 __device__ __noinline__ void exact_word(const T* src, float z, float s, int32_t* dst) {
   const Coder c(z, s);
@@ -233,8 +235,8 @@ __device__ __noinline__ void exact_word(const T* src, float z, float s, int32_t*
     const float q = __saturatef(fmaf(x, c.inv, c.shift)) * 15.0f;
     uint32_t code = static_cast<uint32_t>(q + 0.5f);
     if (fabsf(q - rintf(q)) >= c.sure) {
-      const float low = floorf(q);
       const double d = static_cast<double>(x) - static_cast<double>(z);
+      const float low = fminf(fmaxf(floorf(static_cast<float>(d) / s), 0.0f), 14.0f);
       const double border = static_cast<double>((low + 0.5f) * s);
       const uint32_t k = static_cast<uint32_t>(low);
       code = d > border ? k + 1 : (d < border ? k : (k + 1) & ~1u);

@@ -469,6 +469,18 @@ def test_kv4_codes_near_borders(dtype):
     store_case(64, 1, d, 16, dtype, x=x[:, None].to(DEV))
 
 
+@pytest.mark.parametrize("base", [1.0, 1.0003, -3.0007, 100.03, 30000.7])
+def test_kv4_narrow_rows(base):
+    """fp32 rows that are narrow against their offset: the zero's rounding and
+    the quotient's are many steps, and quotients are far beyond 15."""
+    d = 128
+    g = torch.Generator().manual_seed(13)
+    widths = 2.0 ** torch.arange(-24, 2).float()
+    rows = torch.rand(len(widths), 3, d, generator=g, dtype=torch.float64)
+    x = (base + widths.double()[:, None, None] * rows).float()
+    store_case(len(widths), 3, d, 16, torch.float32, x=x.to(DEV))
+
+
 def test_kv4_out_of_range_slots_and_refusals():
     cache = new_cache(2, 16, 2, 64)
     x = torch.randn(4, 2, 64, device=DEV)
