@@ -894,6 +894,8 @@ void check_kv4_rows(const torch::Tensor& key, const torch::Tensor& value,
               ": key and value must have the same shape and dtype");
   check_kv4_cache(kv_cache, dev, who, key.size(1), key.size(2));
   check_index(slot_mapping, dev, who, "slot_mapping", key.size(0), false);
+  TORCH_CHECK(!overlap(key, kv_cache) && !overlap(value, kv_cache), who,
+              ": key or value overlaps kv_cache");
 }
 
 }  // namespace

@@ -512,6 +512,7 @@ def test_kv4_out_of_range_slots_and_refusals():
     bad("int32 or int64", slots_=slots.float())
     bad("must be a CUDA", slots_=slots.cpu())
     bad("dense", key=x.transpose(0, 1), value=x.transpose(0, 1))
+    bad("overlaps kv_cache", value=cache.view(-1)[:512].view(torch.float32).view(4, 2, 64))
     with pytest.raises(RuntimeError, match="overlap"):
         c_ops.kv4_load(cache, slots, out, out)
     packed = torch.full((4, 4 * 64), 9.0, device=DEV)  # key and value side by side
