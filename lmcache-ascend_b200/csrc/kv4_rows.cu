@@ -36,7 +36,9 @@
 //
 // Measured: 4 suffixes of up to 1024 tokens behind prefixes of up to 16384, 64
 // query heads over 8 of 128, bf16: 1150 us, 700 TFLOP/s (0.42 of a plain bf16
-// product). Issue slots bound it (77% used); Q K^T with 64 columns also takes 46
+// product). By its counters no one unit bounds it: 54% of the issue slots, 32% of
+// the tensor pipe. It waits in the chain from S through softmax to P V, of which
+// a CTA has two units' worth under way. Q K^T with 64 columns takes 46
 // cycles of the tensor core where 32 would do (128 columns: 64.5), but two units'
 // S of 128 and O do not fit its memory. On the way: one unit a CTA 1856 us, two
 // 1513, eight softmax warps a unit instead of four 1455, one elected lane in the
