@@ -668,9 +668,10 @@ __device__ __forceinline__ bool produce(const DecodeParams& p, const Line& line,
     uint8_t* to = dst + (r * 32 + lane) * p.tok_stride;
     const int64_t from = static_cast<int64_t>(row[r]) * row_bytes;
     if (p.groups == 1) {
-      // runs of rows that follow one another in the cache: one copy each
+      // runs of rows that follow one another in the cache: one copy each. Row 0
+      // does not follow a token that is not there (-1).
       const int32_t prev = __shfl_up_sync(0xffffffffu, row[r], 1);
-      const bool start = row[r] >= 0 && (lane == 0 || row[r] != prev + 1);
+      const bool start = row[r] >= 0 && (lane == 0 || prev < 0 || row[r] != prev + 1);
       const uint32_t stops = __ballot_sync(0xffffffffu, start) | ~there[r];
       if (start) {
         const uint32_t above = lane == 31 ? 0 : stops >> (lane + 1);
