@@ -64,11 +64,14 @@ __device__ __forceinline__ void raise_flag(unsigned int* status, unsigned int fl
 // per device (the attribute call costs microseconds; later launches only
 // compare against the cached limit). One cache per kernel: Fn is a template
 // argument, not a parameter, so kernels with equal signatures stay distinct.
+// A launch has 48 KB without asking, for static and dynamic shared memory
+// together: 16 KB of dynamic memory leave room for 32 KB of static memory,
+// more than any kernel here has.
 template <auto Fn>
 cudaError_t ensure_smem_limit(size_t bytes, size_t cap) {
   constexpr int kMaxDevices = 64;
   static std::atomic<int> limit[kMaxDevices];
-  if (bytes <= 48 * 1024) return cudaSuccess;
+  if (bytes <= 16 * 1024) return cudaSuccess;
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;

@@ -988,9 +988,7 @@ template <typename T, int D, int NT, int ST>
 cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(p.stages) * p.stage_bytes + merge_bytes(p.heads, NT, D) +
                       (static_cast<size_t>(p.a.batch) + 1) * 4;
-  // 47 KB: the static shared memory counts towards the 48 KB that need no limit
-  cudaError_t err = ensure_smem_limit<kv4_decode_kernel<T, D, NT, ST>>(
-      smem > 47 * 1024 ? smem + 1024 : smem, 224 * 1024);
+  cudaError_t err = ensure_smem_limit<kv4_decode_kernel<T, D, NT, ST>>(smem, 224 * 1024);
   if (err != cudaSuccess) return err;
   kv4_decode_kernel<T, D, NT, ST><<<pl.ctas, kThreads, smem, stream>>>(p);
   err = cudaGetLastError();

@@ -2,6 +2,10 @@
 tables with holes, batch sizes around a launch limit, values and lengths at the
 ends of their types, keys that a query does not see."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -11,6 +15,7 @@ from tests import test_serving_gpu as base
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(autouse=True)
@@ -110,3 +115,25 @@ def test_attention_after_the_free_list_ran_out():
                                     b.scale, [8], 0, 0, 2)
     err = (out.cpu().double() - want).abs()
     assert bool((err <= base.half_step(torch.bfloat16) * (want.abs() + slack) + slack).all())
+
+
+# ---------------------------------------------------------------------------
+# Batches around the shared memory that a launch has without asking
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("slot", ["int64", "int32"])
+@pytest.mark.parametrize("requests", [4074, 4075, 4096, 4097])
+def test_slots_around_the_default_shared_memory(requests, slot):
+    """The sums of 4075 to 4096 requests fill the default shared memory but for
+    what the kernel has besides. In a process of its own: a larger batch before
+    raises the limit for good."""
+    code = ("import sys; sys.path[:0] = sys.argv[1:3]\n"
+            "import numpy as np, torch\n"
+            "from tests import test_serving_gpu as base\n"
+            f"rs = np.random.RandomState({requests})\n"
+            f"base.run_slots(rs.randint(0, 40, {requests}), rs.randint(0, 4, {requests}), 16, 4,"
+            f" st=torch.{slot})\n"
+            "assert base.c_ops.device_status(0) == 0\n")
+    res = subprocess.run([sys.executable, "-c", code, ROOT, os.path.join(ROOT, "lmcache-ascend_b200")],
+                         capture_output=True, text=True, cwd=ROOT, timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]
