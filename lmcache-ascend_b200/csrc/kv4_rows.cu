@@ -6,18 +6,26 @@
 // of one request and KV head; its rows are the lanes of the tensor memory. With
 // a tile of 64 cache tokens:
 //   S = Q Ck^T     tcgen05.mma 128 x 64 x D, Ck the K codes,
-//   t = S sk + zk (sum of q), p = exp2(t a - m),
+//   t = S sk + zk (sum of q), p = exp2(t a + e - m),
 //   O += P V'      tcgen05.mma 128 x D x 64, P from tensor memory.
 // The K codes are exact as in the decode kernel (the fp16 bit patterns c and
 // 16 c, c 2^-24; Q's odd elements carry the 1/16), so a logit is an fp32 sum of
-// exact products. V is made fp16 on the way, v 2^-e with 2^e above the largest
-// of its 16 tokens; P takes the 2^e, relative to the row's own E, so neither
-// loses small caches nor overflows. Both are rounded to fp16 once; for bf16
-// results that is an eighth of their own rounding. fp16 results are rounded no
-// more coarsely than V and P: they take P as two fp16 numbers, p and what its
-// rounding left, in a second product, which leaves V's rounding alone (error
-// against 64 bits 2.9e-4 of the result's size, 2.1e-4 is the result's own, and
-// 3.4e-4 with one number).
+// exact products. V is made fp16 on the way, v 2^-e with the largest of 16 tokens
+// near the end of fp16's range, and P takes the 2^e. Both are rounded to fp16
+// once; for bf16 results that is an eighth of their own rounding. fp16 results
+// are rounded no more coarsely than V and P: they take P as two fp16 numbers, p
+// and what its rounding left, in a second product, which leaves V's rounding
+// alone (error against 64 bits 2.9e-4 of the result's size, 2.1e-4 is the result's
+// own, and 3.4e-4 with one number).
+//   What a row does not see, or gives no weight, costs it nothing as long as its
+// values are within 2^21 of the others': m is the row's own, from the p 2^e of
+// the keys that it sees, so the largest P lies between 2^7 and 2^15 and numbers
+// down to 2^-21 of 2^7 are normal; V is normal down to 2^-28 of the largest of
+// its 16 tokens. Further apart, values in the 16 of a larger one lose bits (2^24
+// apart, those that bf16 does not have). Exact codes as V, with s in P and z in a
+// sum of its own, would not: they took 1370 to 1450 us where this takes 1140, for
+// what every pair of tokens then has to load. So would more head for P cost time:
+// 2^9 instead of 2^7, with more tiles taken again, 1194 us.
 //
 // A CTA has two such units (one for D = 256), 256 query rows, which share the
 // tiles. Per tile the tensor core needs 1024 cycles for them, the exponentials
@@ -31,8 +39,8 @@
 //    from tensor memory, takes the place of its S);
 //  - eight warps a unit compute softmax. A lane has 2 rows x 16 tokens, not one
 //    row x 32 tokens, and so loads half as many of the tokens' scales.
-// O stays in tensor memory; it is rescaled only when a row's reference grows by
-// more than 2^8, which P's range leaves room for.
+// O stays in tensor memory; it is rescaled only when a row's P outgrows 2^15, and
+// its m then leaves room for 2^8 more.
 //
 // Measured: 4 suffixes of up to 1024 tokens behind prefixes of up to 16384, 64
 // query heads over 8 of 128, bf16: 1150 us, 700 TFLOP/s (0.42 of a plain bf16
@@ -56,10 +64,10 @@ namespace {
 
 constexpr int kRows = 128;  // query rows of a unit
 constexpr int kTok = 64;    // cache tokens of a tile
-// How far P may exceed 1 before O is rescaled, log2: by a row's maximum, and
-// by the exponent of V.
-constexpr float kSlack = 8.0f;
-constexpr float kExpSlack = 4.0f;
+// log2 of a row's largest P: what it may grow to before O is rescaled (fp16 ends
+// at 2^16), and what it is then.
+constexpr float kMost = 15.0f;
+constexpr float kHead = 7.0f;
 
 struct RowsParams {
   AttnParams a;
@@ -287,9 +295,8 @@ struct Control {
   uint64_t drained;
   float4 kpar[kMaxStages][kTok / 2];  // tokens 2 i, 2 i + 1: (sk, sk, zk, zk)
   uint32_t valid[kMaxStages][4];      // two bits a token, 16 tokens each
-  float2 vexp[kMaxStages][4];         // e of 16 tokens, twice
+  float4 vexp[kMaxStages][4];         // of 16 tokens: e, twice, and 2^-e
   float2 row[2 * kRows];              // a, sum of q in its unit; at the end m, l
-  float e[2 * kRows];                 // at the end
   uint32_t tmem;
 };
 
@@ -402,27 +409,31 @@ __device__ __forceinline__ __half2 as_half2(uint32_t v) {
   return *reinterpret_cast<const __half2*>(&v);
 }
 
-// Eight values of V in the order 0, 4, 1, 5, 2, 6, 3, 7, of the bit patterns that
-// expand_k makes: c 2^-24 times s 2^24 (or 16 c 2^-24 times s 2^20), plus z,
-// rounded once.
-__device__ __forceinline__ uint4 expand_v(uint32_t w, __half2 s24, __half2 s20, __half2 z) {
-  const uint32_t x = w >> 8;
-  return make_uint4(half2_bits(__hfma2(as_half2(w & 0x000f000fu), s24, z)),
-                    half2_bits(__hfma2(as_half2(w & 0x00f000f0u), s20, z)),
-                    half2_bits(__hfma2(as_half2(x & 0x000f000fu), s24, z)),
-                    half2_bits(__hfma2(as_half2(x & 0x00f000f0u), s20, z)));
+// Codes as normal numbers, exactly: on top of 1024, less 1024.
+__device__ __forceinline__ __half2 normal(uint32_t bits) {
+  return __hsub2(as_half2(bits | 0x64006400u), __half2half2(__ushort_as_half(0x6400)));
 }
 
-// fp16 results take normal numbers, c and 16 c on top of 1024 less 1024: the
-// matrix unit cuts off bits of sums of subnormals (codes in the decode kernel).
+// Eight values of V in the order 0, 4, 1, 5, 2, 6, 3, 7: s c + z, or s16 16 c + z,
+// rounded once.
+__device__ __forceinline__ uint4 expand_v(uint32_t w, __half2 s, __half2 s16, __half2 z) {
+  const uint32_t x = w >> 8;
+  return make_uint4(half2_bits(__hfma2(normal(w & 0x000f000fu), s, z)),
+                    half2_bits(__hfma2(normal(w & 0x00f000f0u), s16, z)),
+                    half2_bits(__hfma2(normal(x & 0x000f000fu), s, z)),
+                    half2_bits(__hfma2(normal(x & 0x00f000f0u), s16, z)));
+}
+
+// Eight codes of K in the same order, the odd ones times 16, as their bits lie:
+// c 2^-24. fp16 results take normal numbers: the matrix unit cuts off bits of sums
+// of subnormals (codes in the decode kernel).
 template <bool kNormal>
 __device__ __forceinline__ uint4 expand_k(uint32_t w) {
   const uint32_t x = w >> 8;
   uint32_t r[4] = {w & 0x000f000fu, w & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u};
   if constexpr (kNormal) {
-    const __half2 base = __half2half2(__ushort_as_half(0x6400));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = half2_bits(__hsub2(as_half2(r[j] | 0x64006400u), base));
+    for (int j = 0; j < 4; ++j) r[j] = half2_bits(normal(r[j]));
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -469,17 +480,19 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     const Codes<D> c = next;
     fetch<D>(p, k_head, par, row_in(i + 1, page), lane, next);
     page = page_of(i + 2);
-    // The exponent 8 above the largest value of these 16 tokens: a value's span
-    // is below 2^-7 then, s 2^24 below 2^14. What is lost, with the smallest
-    // values of the 16, is 2^-17 of the largest.
-    const float s = half_lo(c.vpar), z = half_hi(c.vpar);
+    // e places the largest value of these 16 tokens between 2^14 and 2^15. A row
+    // whose parameters are no finite numbers (kv4_store writes none) gives NaN, by
+    // its K, to the queries that see it, and nothing to its neighbours.
+    float s = half_lo(c.vpar), z = half_hi(c.vpar);
+    const bool finite = fabsf(s) <= 65504.0f && fabsf(z) <= 65504.0f;
+    if (!finite) s = z = 0.0f;
     const float most = fmaxf(fabsf(z), fabsf(fmaf(15.0f, s, z)));
     const int e = static_cast<int>(__reduce_max_sync(
-                      0xffffffffu, max((__float_as_uint(most) >> 23) & 255u, 80u))) - 118;
+                      0xffffffffu, max((__float_as_uint(most) >> 23) & 255u, 80u))) - 141;
     const float down = pow2i(-e);
-    const __half2 s24 = __half2half2(__float2half_rn(s * down * 16777216.0f));
-    const __half2 s20 = __half2half2(__float2half_rn(s * down * 1048576.0f));
-    const __half2 z2 = __half2half2(__float2half_rn(z * down));
+    const __half2 vs = __half2half2(__float2half_rn(s * down));
+    const __half2 vs16 = __half2half2(__float2half_rn(s * down * 0.0625f));
+    const __half2 vz = __half2half2(__float2half_rn(z * down));
     const uint32_t there = __ballot_sync(0xffffffffu, c.there);
     if (i >= L::kStages && !mbar_wait(&ctl.free[stage], phase)) return false;
     uint8_t* k = smem + stage * L::kStage;
@@ -492,17 +505,18 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
       for (int j = 0; j < 4; ++j) {
         uint8_t* to = k + n * L::kPanel + swizzled(tok, piece + j);
         *reinterpret_cast<uint4*>(to) = expand_k<kNormal>(kw[j]);
-        *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], s24, s20, z2);
+        *reinterpret_cast<uint4*>(to + L::kV) = expand_v(vw[j], vs, vs16, vz);
       }
     }
     if (lane % 2 == 0) {
       float* to = reinterpret_cast<float*>(&ctl.kpar[stage][tok / 2]) + tok % 2;
-      to[0] = half_lo(c.kpar);
+      to[0] = finite ? half_lo(c.kpar) : __int_as_float(0x7fffffff);
       to[2] = half_hi(c.kpar);
     }
     if (lane == 0) {
       ctl.valid[stage][w] = there;
-      ctl.vexp[stage][w] = make_float2(static_cast<float>(e), static_cast<float>(e));
+      ctl.vexp[stage][w] =
+          make_float4(static_cast<float>(e), static_cast<float>(e), down, down);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -610,41 +624,39 @@ struct Part {
   float a[2];
   uint64_t qsum[2];     // rows' factors, the second twice
   float m[2];           // references (log2)
-  float top[2];         // largest t of this tile
+  float top[2];         // largest t a + e of this tile
   float l[2];           // sums of this tile, in units of 2^m
   int32_t hi[2];        // last key seen, as a virtual token
 };
 
-// S into P and the rows' largest t and sums. `ve` are the exponents of V's 16
-// tokens each, `e` the warp's.
+// S into P and the rows' largest t a + e and sums.
 template <bool kAll, bool kTwo>
 __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_cols,
                                              const ulonglong2* kpar, const uint32_t* valid,
-                                             const float2* vexp, int32_t v0, float e, Part& part,
+                                             const ulonglong2* vexp, int32_t v0, Part& part,
                                              uint32_t (&pr)[16], uint32_t (&rest)[16]) {
   const int t4 = threadIdx.x % 4;
   uint32_t s[32];
   tmem_load_rows(s, s_cols);
   uint64_t back_ref[2], a2[2];
-  float top[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float r = -(part.m[k] + e);
-    back_ref[k] = pair(r, r);
+    back_ref[k] = pair(-part.m[k], -part.m[k]);
     a2[k] = pair(part.a[k], part.a[k]);
-    top[k] = -INFINITY;
+    part.top[k] = -INFINITY;
     part.l[k] = 0.0f;
   }
   tmem_wait_load(s);
 #pragma unroll
   for (int n = 0; n < 4; ++n) {  // 16 tokens: one exponent of V
-    const uint64_t ve = *reinterpret_cast<const uint64_t*>(&vexp[n]);
-    const float back = exp2_approx(e - unpair(ve).x);  // to the units of l
+    const ulonglong2 ve = vexp[n];
+    const float back = unpair(ve.y).x;  // to the units of l
     const ulonglong2 kp[2] = {kpar[8 * n + t4], kpar[8 * n + 4 + t4]};  // (sk, sk), (zk, zk)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const uint64_t ref = add2(ve, back_ref[k]);
+      const uint64_t ref = add2(ve.x, back_ref[k]);
       float2 x[2];
+      float top = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = 8 * n + 4 * h + 2 * k;
@@ -662,7 +674,7 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
           t.y = seen(v + 1, there >> 2) ? t.y : -INFINITY;
           t2 = pair(t.x, t.y);
         }
-        top[k] = fmaxf(top[k], fmaxf(t.x, t.y));
+        top = fmaxf(top, fmaxf(t.x, t.y));
         x[h] = unpair(fma2(t2, a2[k], ref));
         x[h].x = exp2_approx(x[h].x);
         x[h].y = exp2_approx(x[h].y);
@@ -674,18 +686,16 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
       }
       const float2 sum = unpair(add2(pair(x[0].x, x[0].y), pair(x[1].x, x[1].y)));
       part.l[k] = fmaf(sum.x + sum.y, back, part.l[k]);
+      part.top[k] = fmaxf(part.top[k], fmaf(top, part.a[k], unpair(ve.x).x));
     }
   }
-  part.top[0] = top[0];
-  part.top[1] = top[1];
 }
 
 // A warp has 16 of a unit's rows: warps w and w + 4 have those of tensor memory
-// lanes 32 w ..., 16 each. Sums l are in units of 2^m, O in units of 2^(m + e),
-// e the same for all rows of a warp. P is taken with the references that are
-// there; only a tile that outgrows them by the slack (the first one, and few
-// after it) is taken again, with new ones. So nothing waits for a tile's
-// maximum, and a thread never holds more than the tile's S.
+// lanes 32 w ..., 16 each. l and O are in units of 2^m, a row's own. P is taken
+// with the references that are there; only a tile that outgrows them (the first
+// one, and few after it) is taken again, with new ones. So nothing waits for a
+// tile's maximum, and a thread never holds more than the tile's S.
 template <int D, bool kTwo>
 __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& range, int32_t t0,
                                        int32_t tiles, int32_t pos_first, int32_t pos_last,
@@ -713,7 +723,6 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     const int tok = static_cast<int>(p.div_group.div(static_cast<uint32_t>(first_row + row)));
     part.hi[k] = tok < rq.n ? rq.len - rq.n + tok + to_v : -1;
   }
-  float e = -100.0f;
   bool ok = true;
   int stage = 0;
   uint32_t phase = 0;
@@ -727,44 +736,33 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     const uint32_t s_cols = mine + (i & 1) * kTok;
     // is every key of the tile there and seen by every row?
     const int32_t v0 = (t0 + i) * kTok;
-    bool all;
-    float vmax;
-    {
-      const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
-      all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu && v0 + kTok - 1 <= hi_first &&
-            (p.window == 0 || v0 > hi_last - p.window || v0 + kTok - 1 < p.sinks);
-      const float2* ve = ctl.vexp[stage];
-      vmax = fmaxf(fmaxf(ve[0].x, ve[1].x), fmaxf(ve[2].x, ve[3].x));
-    }
+    const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
+    const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu &&
+                     v0 + kTok - 1 <= hi_first &&
+                     (p.window == 0 || v0 > hi_last - p.window || v0 + kTok - 1 < p.sinks);
+    const ulonglong2* kpar = reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]);
+    const ulonglong2* vexp = reinterpret_cast<const ulonglong2*>(ctl.vexp[stage]);
     uint32_t pr[16], rest[16];
     for (;;) {
       if (all) {
-        softmax_tile<true, kTwo>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
-                           part, pr, rest);
+        softmax_tile<true, kTwo>(p, s_cols, kpar, ctl.valid[stage], vexp, v0, part, pr, rest);
       } else {
-        softmax_tile<false, kTwo>(p, s_cols, reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]), ctl.valid[stage], ctl.vexp[stage], v0, e,
-                            part, pr, rest);
+        softmax_tile<false, kTwo>(p, s_cols, kpar, ctl.valid[stage], vexp, v0, part, pr, rest);
       }
-      bool grow = vmax - e > kExpSlack;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        part.top[k] *= part.a[k];
-        grow = grow || part.top[k] - part.m[k] > kSlack;
+      if (!__any_sync(0xffffffffu, part.top[0] - part.m[0] > kMost ||
+                                       part.top[1] - part.m[1] > kMost)) {
+        break;
       }
-      if (!__any_sync(0xffffffffu, grow)) break;
-      const float e_new = fmaxf(e, vmax);
-      const float down = exp2_approx(e - e_new);
-      e = e_new;
       float alpha[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        part.top[k] = fmaxf(part.top[k], __shfl_xor_sync(0xffffffffu, part.top[k], 1));
-        part.top[k] = fmaxf(part.top[k], __shfl_xor_sync(0xffffffffu, part.top[k], 2));
-        const float m_new = fmaxf(part.m[k], part.top[k]);
-        const float f = exp2_approx(part.m[k] - m_new);
+        float top = part.top[k];
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = top - part.m[k] > kMost ? top - kHead : part.m[k];
+        alpha[k] = exp2_approx(part.m[k] - m_new);
         part.m[k] = m_new;
-        l[k] *= f;
-        alpha[k] = f * down;
+        l[k] *= alpha[k];
       }
       if (i > 0) {
         ok = mbar_wait(&ctl.pvdone[unit], (i - 1) & 1) && ok;
@@ -802,7 +800,6 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
     if (t4 == 0) {
       ctl.row[warp_row + g + 8 * k] = make_float2(part.m[k], l[k]);
-      ctl.e[warp_row + g + 8 * k] = e;
     }
   }
   return ok;
@@ -810,15 +807,14 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
 
 template <typename T, int D>
 __device__ __forceinline__ void write_row(const RowsParams& p, const Request& rq, int flat,
-                                          int kv_head, float* part, float2 ml, float e, bool any,
+                                          int kv_head, float* part, float2 ml, bool any,
                                           uint32_t mine, int c0, int c1) {
   using L = Layout<D>;
   const AttnParams& a = p.a;
   const int tok = static_cast<int>(a.div_group.div(static_cast<uint32_t>(flat)));
   const bool there = tok < rq.n;
   const int head = kv_head * a.group + (flat - tok * a.group);
-  const float unit = exp2_approx(e);
-  const float f = part == nullptr ? inverse_sum(ml.y) * unit : unit;
+  const float f = part == nullptr ? inverse_sum(ml.y) : 1.0f;
   T* dst = static_cast<T*>(a.out) + (rq.row0 + static_cast<int64_t>(tok)) * a.out_stride +
            static_cast<int64_t>(head) * D;
 #pragma unroll 1
@@ -943,7 +939,7 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
       const int64_t at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * p.row_tiles + tile;
       part = p.part + ((at * p.splits + split) * kCtaRows + cta_row) * (D + 4);
     }
-    write_row<T, D>(p, rq, flat, kv_head, part, ctl.row[cta_row], ctl.e[cta_row], t1 > t0, mine,
+    write_row<T, D>(p, rq, flat, kv_head, part, ctl.row[cta_row], t1 > t0, mine,
                     side * (D / 2), (side + 1) * (D / 2));
   }
   fence_before();

@@ -137,3 +137,162 @@ def test_slots_around_the_default_shared_memory(requests, slot):
     res = subprocess.run([sys.executable, "-c", code, ROOT, os.path.join(ROOT, "lmcache-ascend_b200")],
                          capture_output=True, text=True, cwd=ROOT, timeout=300)
     assert res.returncode == 0, res.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------------
+# Many query rows: V of keys that a query does not see or gives no weight
+# ---------------------------------------------------------------------------
+
+def fill(b, r, half, codes, scale, zero):
+    """Request r's rows of one half become these."""
+    words = ref.kv4_words(codes, scale, zero)
+    tok = torch.arange(codes.shape[0])
+    slot = b.table[r].cpu().long()[tok // b.bs] * b.bs + tok % b.bs
+    b.cache[half].view(-1, b.cache.shape[-1])[slot.to(DEV), : words.shape[1]] = words.to(DEV)
+    b.codes[r][half], b.params[r][half] = codes, (scale, zero)
+
+
+def weighted_bound(b, r, rows, want, window, sinks, spread):
+    """What the result of each query row may be off by. Unlike the oracle's own
+    bound it counts every key by its weight p, so that a key without weight has
+    no share in it: V and P are rounded to fp16 (2^-11 each of sum p |v|); logits
+    are off by d = 4 * 2^-19 of their terms, which moves the result by sum p d (v
+    - result); (keys / 16 + 8) roundings of 2^-22 of sum p (|v| + 15 s). A P that
+    is no normal number is off by 2^-25 where the row's largest is above 2^7; 16
+    tokens with a value `spread` times theirs among them have it that much
+    smaller."""
+    n, length = b.qlens[r], b.lens[r]
+    at = sum(b.qlens[:r])
+    k, v = (ref.kv4_values(b.codes[r][i], *b.params[r][i]) for i in range(2))
+    s = b.params[r][1][0]
+    kabs = b.params[r][0][0][..., None] * 15 + b.params[r][0][1].abs()[..., None]
+    out = torch.zeros_like(want)
+    for i, row in enumerate(rows):
+        seen = ref.visible(length - n + row, torch.arange(length), window, sinks)
+        for h in range(b.hkv * b.group):
+            kv = h // b.group
+            x = b.q[at + row, h].cpu().double()
+            p = torch.softmax((k[seen, kv] @ x) * b.scale, 0)
+            mass = (kabs[seen, kv] * x.abs()).sum(-1) * abs(b.scale)
+            big = v[seen, kv].abs()
+            size = big + 15 * s[seen, kv, None] + want[i, h].abs()
+            steps = (int(seen.sum()) / 16 + 8) * 2.0**-22
+            out[i, h] = (2.0**-10 * (p @ big) + (p * (4 * mass * 2.0**-19 + steps)) @ size
+                         + 2.0**-32 * spread * p.max() * (big * (p[:, None] > 2.0**-60)).sum(0))
+    return out
+
+
+def check_rows(b, out, r, rows, window=0, sinks=0, spread=1.0):
+    at, n = sum(b.qlens[:r]), b.qlens[r]
+    pos = [b.lens[r] - n + i for i in rows]
+    want, _ = ref.kv4_attention(b.q[at : at + n].cpu()[rows], b.codes[r], b.params[r], b.scale, pos,
+                                window, sinks, b.hkv)
+    slack = weighted_bound(b, r, rows, want, window, sinks, spread)
+    err = (out[at : at + n].cpu().double()[rows] - want).abs()
+    bound = base.half_step(b.dtype) * (want.abs() + slack) + slack + 2.0**-25
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("power", [8, 10, 13, 17, 20])
+def test_rows_large_value_out_of_sight(dtype, d, power):
+    """The value of a key behind a query's position, or in front of its window,
+    2^power times its neighbours': the query's row, which lives on those
+    neighbours, is as good as without it."""
+    n = 60
+    for key, window, rows in ((8, 0, range(8)), (41, 0, range(32, 41)), (8, 5, range(13, 16)),
+                              (8, 5, range(40, 60))):
+        b = base.Batch([n], [n], 1, 2, d, 16, dtype, seed=d, std=2.0**-7)
+        codes, (scale, zero) = b.codes[0][1], b.params[0][1]
+        scale[key] = (scale[key] * 2.0**power).half().double()
+        zero[key] = (zero[key] * 2.0**power).half().double()
+        fill(b, 0, 1, codes, scale, zero)
+        out = b.run(window, 0)
+        check_rows(b, out, 0, list(rows), window, spread=2.0**power)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("power", [8, 10, 13, 17, 20])
+@pytest.mark.parametrize("key", [0, 37, 410])
+def test_rows_large_value_without_weight(dtype, d, power, key):
+    """A key that every query sees and gives no weight, with a value 2^power
+    times the others': the rows are as good as without it."""
+    n, q = 430, 24
+    b = base.Batch([n], [q], 1, 2, d, 16, dtype, seed=d + power, std=2.0**-7)
+    codes, (scale, zero) = b.codes[0][1], b.params[0][1]
+    scale[key] = (scale[key] * 2.0**power).half().double()
+    zero[key] = (zero[key] * 2.0**power).half().double()
+    assert float(scale.max()) < 65504 and float(zero.abs().max()) < 65504
+    fill(b, 0, 1, codes, scale, zero)
+    kc, (ks, kz) = b.codes[0][0], b.params[0][0]
+    kz[key], ks[key], kc[key] = -60000.0, 2.0**-7, 0
+    fill(b, 0, 0, kc, ks, kz)
+    b.q[:, :, 1:] *= 0.01
+    b.q[:, :, 0] = 8.0
+    b.q[:] = b.q.abs()  # the logits of that key are far below the others'
+    check_rows(b, b.run(), 0, [0, 1, 11, 23], spread=2.0**power)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_not_finite_out_of_sight(dtype):
+    """A value row that is no number (a page not made by kv4_store) spoils the
+    queries that see it and no others."""
+    n = 60
+    b = base.Batch([n], [n], 1, 2, 128, 16, dtype)
+    good = b.run()
+    for key in (8, 41):
+        slot = int(b.table[0, key // 16]) * 16 + key % 16
+        word = b.cache[1].view(-1, b.cache.shape[-1])[slot]
+        keep = int(word[16])
+        for bad in (0x7E00, 0x7C00, 0x7E000000, 0x7C000000):  # s or z, NaN or infinite
+            word[16] = bad
+            out = b.run()
+            assert bool(out[key:].isnan().all()) or bool((~out[key:].isfinite()).all())
+            check_rows(b, out, 0, list(range(key)))
+        word[16] = keep
+    assert torch.equal(b.run(), good)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_scales_that_differ_by_powers(dtype, d):
+    """Value scales that grow and shrink by many powers of two along the cache,
+    and rows of one value only (scale 0), with many query rows."""
+    n, q = 300, 40
+    b = base.Batch([n], [q], 1, 2, d, 16, dtype)
+    g = torch.Generator().manual_seed(2)
+    for half in range(2):
+        codes = torch.randint(0, 16, (n, 1, d), generator=g)
+        e = torch.randint(-14, 6, (n, 1), generator=g).double()
+        scale = (2.0**e) if half else torch.full((n, 1), 0.05, dtype=torch.float64)
+        scale[5::9] = 0
+        codes[5::9] = 0
+        zero = torch.randn(n, 1, generator=g).half().double()
+        fill(b, 0, half, codes, scale, zero)
+    check_rows(b, b.run(), 0, [0, 1, 15, 16, 39], spread=2.0**19)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("std,shift", [(1e-4, 0.0), (300.0, 0.0), (0.01, 5.0), (1.0, -40.0)])
+def test_rows_value_ranges(dtype, std, shift):
+    """Small, large and shifted caches with many query rows."""
+    b = base.Batch([90, 300], [30, 50], 2, 4, 128, 16, dtype, std=std, shift=shift)
+    if std > 10:
+        b.scale = 1e-5
+    out = b.run()
+    for r in range(2):
+        check_rows(b, out, r, [0, 7, 29])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_of_one_value(d):
+    """Caches whose rows hold one value each (scale 0), down to the smallest."""
+    n, q = 150, 30
+    b = base.Batch([n], [q], 1, 2, d, 16, torch.float16)
+    for value in (0.0, 2.0**-24, -3.0, 65504.0):
+        zero = torch.full((n, 1), value, dtype=torch.float64)
+        fill(b, 0, 1, torch.zeros(n, 1, d, dtype=torch.long), torch.zeros_like(zero), zero)
+        out = b.run()
+        assert bool((out == value).all())
