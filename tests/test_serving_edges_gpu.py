@@ -296,3 +296,25 @@ def test_rows_of_one_value(d):
         fill(b, 0, 1, torch.zeros(n, 1, d, dtype=torch.long), torch.zeros_like(zero), zero)
         out = b.run()
         assert bool((out == value).all())
+
+
+# ---------------------------------------------------------------------------
+# kv4_store: the scale is a fifteenth, rounded once to fp32 and once to fp16
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exponent", [-12, 0, 13])
+def test_kv4_scale_is_a_fifteenth(exponent):
+    """Every fp32 span of a binade: rows [0, span, ...], whose scale is the fp32
+    quotient span / 15, rounded to fp16."""
+    n, d = 1 << 23, 8
+    span = torch.arange(n, device=DEV, dtype=torch.int32).add_((127 + exponent) << 23).view(
+        torch.float32)
+    x = torch.zeros(n, 1, d, device=DEV)
+    x[:, 0, 3] = span
+    cache = torch.full((2, n // 16, 16, 1, ref.kv4_row_words(1, d)), -1, dtype=torch.int32,
+                       device=DEV)
+    c_ops.kv4_store(x, x, cache, torch.arange(n, device=DEV, dtype=torch.int32))
+    want = (span.double() / 15.0).float().half()  # 53 bits hold a 24-bit quotient: rounded once
+    got = cache[0].view(n, -1)[:, 1].contiguous().view(torch.float16)[::2]
+    assert torch.equal(got, want)
+    assert torch.equal(cache[0], cache[1])
