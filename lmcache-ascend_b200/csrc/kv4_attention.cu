@@ -355,8 +355,7 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
           if (mask) {
             const int32_t key = key_of(range, v0 + first + u * 16 + i * 8 + sigma(g));
             const int32_t ps = q.pos[n][col];
-            seen = seen && key <= ps &&
-                   (p.a.window == 0 || key > ps - p.a.window || key < p.a.sinks);
+            seen = seen && key <= ps && (key > window_end(p.a, ps) || key < p.a.sinks);
           }
           v = seen ? v : -INFINITY;
         }

@@ -76,6 +76,12 @@ __device__ __forceinline__ Request load_request(const AttnParams& p, int b, bool
   return r;
 }
 
+// The last key that a query at `pos` (which may lie before the first key) does
+// not see for its window; -1: none. Never below -1, whatever the two are.
+__device__ __forceinline__ int32_t window_end(const AttnParams& p, int32_t pos) {
+  return p.window > 0 && pos >= p.window ? pos - p.window : -1;
+}
+
 // The keys that any query of a run of positions [p0, p1] sees, as one virtual
 // range [0, count): first `head` first tokens, then the tokens from `first` on.
 struct KeyRange {
@@ -85,7 +91,7 @@ struct KeyRange {
 __device__ __forceinline__ KeyRange key_range(const AttnParams& p, int32_t p0, int32_t p1) {
   KeyRange k;
   if (p1 < 0) return KeyRange{0, 0, 0};
-  k.first = p.window > 0 && p0 - p.window + 1 > 0 ? p0 - p.window + 1 : 0;
+  k.first = window_end(p, p0) + 1;
   k.head = min(p.sinks, k.first);
   k.count = k.head + p1 + 1 - k.first;
   return k;

@@ -668,7 +668,7 @@ __device__ __forceinline__ void softmax_tile(const AttnParams& p, uint32_t s_col
           const uint32_t there = valid[n] >> (2 * (col % 16));
           const auto seen = [&](int32_t at_v, uint32_t bit) {
             return at_v <= part.hi[k] &&
-                   (p.window == 0 || at_v > part.hi[k] - p.window || at_v < p.sinks) && (bit & 1);
+                   (at_v > window_end(p, part.hi[k]) || at_v < p.sinks) && (bit & 1);
           };
           t.x = seen(v, there) ? t.x : -INFINITY;
           t.y = seen(v + 1, there >> 2) ? t.y : -INFINITY;
@@ -707,7 +707,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
   const int warp_row = unit * kRows + lanes;                // of the CTA's rows
   const uint32_t mine = ctl.tmem + unit * L::kUnit + (static_cast<uint32_t>(lanes) << 16);
   // Visible keys of a row at position i, as virtual tokens (KeyRange): v <= hi,
-  // and with a window v > hi - window or v < sinks.
+  // and v > window_end(hi) or v < sinks.
   const int32_t to_v = range.head - range.first;
   const int32_t hi_first = pos_first + to_v, hi_last = pos_last + to_v;
   Part part;
@@ -739,7 +739,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     const uint4 valid = *reinterpret_cast<const uint4*>(ctl.valid[stage]);
     const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu &&
                      v0 + kTok - 1 <= hi_first &&
-                     (p.window == 0 || v0 > hi_last - p.window || v0 + kTok - 1 < p.sinks);
+                     (v0 > window_end(p, hi_last) || v0 + kTok - 1 < p.sinks);
     const ulonglong2* kpar = reinterpret_cast<const ulonglong2*>(ctl.kpar[stage]);
     const ulonglong2* vexp = reinterpret_cast<const ulonglong2*>(ctl.vexp[stage]);
     uint32_t pr[16], rest[16];

@@ -318,3 +318,20 @@ def test_kv4_scale_is_a_fifteenth(exponent):
     got = cache[0].view(n, -1)[:, 1].contiguous().view(torch.float16)[::2]
     assert torch.equal(got, want)
     assert torch.equal(cache[0], cache[1])
+
+
+# ---------------------------------------------------------------------------
+# The widest windows, and queries before the cache
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 2, 2**31 - 40, 2**30, 7])
+@pytest.mark.parametrize("qlen,length", [(8, 5), (4, 1), (3, 0), (70, 30), (200, 130)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_window_with_queries_before_the_cache(window, qlen, length, d, dtype):
+    """More queries than tokens under a window of any width: queries before
+    position 0 give zeros, the others see their keys."""
+    b = base.Batch([length, 50], [qlen, 2], 1, 2, d, 16, dtype, seed=qlen)
+    out = b.run(window, 3)
+    b.check(out, window, 3, rows=list(range(0, qlen, 7)) + [-1, -2, -3, qlen - length])
+    assert bool((out[: qlen - length] == 0).all())
+    assert c_ops.device_status(0) == 0
