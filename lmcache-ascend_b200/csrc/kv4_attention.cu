@@ -646,7 +646,7 @@ __device__ __forceinline__ bool produce(const DecodeParams& p, const Line& line,
   const uint32_t par_at = par & ~15u;
   const uint32_t par_bytes = ((par + heads * 4 + 15) & ~15u) - par_at;
   const uint32_t tok_bytes = 2 * (p.groups == 1 ? row_bytes : code_bytes + par_bytes);
-  if (turn > 0 && !mbar_wait(&ring.empty[stage], (turn - 1) & 1)) return false;
+  if (turn > 0 && !warp_wait(&ring.empty[stage], (turn - 1) & 1)) return false;
   uint64_t* full = &ring.full[stage];
   if (lane == 0) {
 #pragma unroll
@@ -734,7 +734,7 @@ __device__ __forceinline__ bool run_line(const DecodeParams& p, const Line& line
       if (j > 0 && j % kWarps == static_cast<uint32_t>(warp) && j - 1 + p.stages < count && ok) {
         ok = produce(p, line, j - 1 + p.stages, data, ring, D / 2);
       }
-      ok = ok && mbar_wait(&ring.full[stage], phase);
+      ok = ok && warp_wait(&ring.full[stage], phase);
       if (working && ok) {
         const uint8_t* at = data + stage * p.stage_bytes;
         bool all = !mask;

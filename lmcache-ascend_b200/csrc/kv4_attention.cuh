@@ -247,9 +247,22 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // LMCB_DEVICE_FLAG_WAIT_TIMEOUT and leaves.
 constexpr uint32_t kWaitLimit = 1u << 22;
 
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
+                                          uint32_t limit = kWaitLimit) {
+  for (uint32_t i = 0; i < limit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
+  }
+  return false;
+}
+
+// The same for a whole warp, whose lanes are told the same: were each to poll for
+// itself, a phase that ends as the last polls go out could send them different
+// ways, in front of instructions that take the whole warp. `limit` is the same for
+// all.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
+                                          uint32_t limit = kWaitLimit) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   }
   return false;
 }

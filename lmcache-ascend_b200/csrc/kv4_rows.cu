@@ -35,7 +35,7 @@
 //  - four warps bring the codes from the pages and expand them into a ring of
 //    stages (128-byte swizzle; a lane's 16-byte pieces of 4 tokens x 2 halves of
 //    a panel hit all banks), ahead of the products;
-//  - one warp issues products, Q K^T a tile ahead of P V, into one of two S (P,
+//  - one thread issues products, Q K^T a tile ahead of P V, into one of two S (P,
 //    from tensor memory, takes the place of its S);
 //  - eight warps a unit compute softmax. A lane has 2 rows x 16 tokens, not one
 //    row x 32 tokens, and so loads half as many of the tokens' scales.
@@ -494,7 +494,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
     const __half2 vs16 = __half2half2(__float2half_rn(s * down * 0.0625f));
     const __half2 vz = __half2half2(__float2half_rn(z * down));
     const uint32_t there = __ballot_sync(0xffffffffu, c.there);
-    if (i >= L::kStages && !mbar_wait(&ctl.free[stage], phase)) return false;
+    if (i >= L::kStages && !warp_wait(&ctl.free[stage], phase)) return false;
     uint8_t* k = smem + stage * L::kStage;
     const uint32_t piece = (lane % 2) * 4;
 #pragma unroll
@@ -527,7 +527,7 @@ __device__ __forceinline__ bool bring(const AttnParams& p, const KeyRange& range
 }
 
 // ---------------------------------------------------------------------------
-// The warp that issues the products
+// The thread that issues the products
 // ---------------------------------------------------------------------------
 
 template <int D>
@@ -568,11 +568,8 @@ struct Issuer {
     if (!mbar_wait(&ctl.full[stage], (j / L::kStages) & 1)) return false;
     if (j >= 2 && !mbar_wait(&ctl.pvdone[u], j & 1)) return false;
     fence_after();
-    if (elect_one()) {
-      issue_qk<D>(tmem + u * L::kUnit + buf * kTok, rows + u * L::kQ, stages + stage * L::kStage);
-      commit(&ctl.sready[u][buf]);
-    }
-    __syncwarp();
+    issue_qk<D>(tmem + u * L::kUnit + buf * kTok, rows + u * L::kQ, stages + stage * L::kStage);
+    commit(&ctl.sready[u][buf]);
     return true;
   }
 
@@ -580,16 +577,13 @@ struct Issuer {
     const int stage = j % L::kStages, buf = j & 1;
     if (!mbar_wait(&ctl.pready[u][buf], (j >> 1) & 1)) return false;
     fence_after();
-    if (elect_one()) {
-      const uint32_t unit = tmem + u * L::kUnit, p = unit + buf * kTok;
-      issue_pv<D>(unit + L::kO, p, stages + stage * L::kStage, j > 0);
-      if constexpr (kTwo) {
-        issue_pv<D>(unit + L::kO, p + kTok / 2, stages + stage * L::kStage, true);
-      }
-      commit(&ctl.pvdone[u]);
-      if (u == units - 1) commit(&ctl.free[stage]);
+    const uint32_t unit = tmem + u * L::kUnit, p = unit + buf * kTok;
+    issue_pv<D>(unit + L::kO, p, stages + stage * L::kStage, j > 0);
+    if constexpr (kTwo) {
+      issue_pv<D>(unit + L::kO, p + kTok / 2, stages + stage * L::kStage, true);
     }
-    __syncwarp();
+    commit(&ctl.pvdone[u]);
+    if (u == units - 1) commit(&ctl.free[stage]);
     return true;
   }
 
@@ -727,8 +721,8 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
   int stage = 0;
   uint32_t phase = 0;
   for (int32_t i = 0; i < tiles; ++i) {
-    if (!mbar_wait(&ctl.full[stage], phase) ||
-        !mbar_wait(&ctl.sready[unit][i & 1], (i >> 1) & 1)) {
+    if (!warp_wait(&ctl.full[stage], phase) ||
+        !warp_wait(&ctl.sready[unit][i & 1], (i >> 1) & 1)) {
       ok = false;
       break;
     }
@@ -765,7 +759,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
         l[k] *= alpha[k];
       }
       if (i > 0) {
-        ok = mbar_wait(&ctl.pvdone[unit], (i - 1) & 1) && ok;
+        ok = warp_wait(&ctl.pvdone[unit], (i - 1) & 1) && ok;
         fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -791,7 +785,7 @@ __device__ __forceinline__ bool attend(const AttnParams& p, const KeyRange& rang
     if (++stage == L::kStages) stage = 0, phase ^= 1;
   }
   if (tiles > 0 && ok) {
-    ok = mbar_wait(&ctl.pvdone[unit], (tiles - 1) & 1);  // the last product
+    ok = warp_wait(&ctl.pvdone[unit], (tiles - 1) & 1);  // the last product
     fence_after();
   }
 #pragma unroll
@@ -925,7 +919,10 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == L::kIssue) {
       const uint32_t q = smem_u32(smem);
-      ok = Issuer<D, kTwo>{ctl.tmem, q, q + L::kUnits * L::kQ, units, ctl}.run(t1 - t0);
+      if (elect_one()) {  // always the same lane: commits track what their thread issued
+        ok = Issuer<D, kTwo>{ctl.tmem, q, q + L::kUnits * L::kQ, units, ctl}.run(t1 - t0);
+      }
+      __syncwarp();
     }
   } else if (warp >= L::kBring) {
     if (L::kUnits == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -944,7 +941,7 @@ kv4_rows_kernel(const __grid_constant__ RowsParams p) {
   }
   fence_before();
   if (__syncthreads_or(!ok)) {
-    if (threadIdx.x == L::kIssue * 32) {
+    if (warp == L::kIssue && elect_one()) {
       raise_flag(a.status, LMCB_DEVICE_FLAG_WAIT_TIMEOUT);
       commit(&ctl.drained);  // products in flight end before their memory is given back
       mbar_wait(&ctl.drained, 0);

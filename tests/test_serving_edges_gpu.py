@@ -2,7 +2,9 @@
 tables with holes, batch sizes around a launch limit, values and lengths at the
 ends of their types, keys that a query does not see."""
 
+import ctypes
 import os
+import shutil
 import subprocess
 import sys
 
@@ -335,3 +337,56 @@ def test_window_with_queries_before_the_cache(window, qlen, length, d, dtype):
     b.check(out, window, 3, rows=list(range(0, qlen, 7)) + [-1, -2, -3, qlen - length])
     assert bool((out[: qlen - length] == 0).all())
     assert c_ops.device_status(0) == 0
+
+
+# ---------------------------------------------------------------------------
+# Waits that give up
+# ---------------------------------------------------------------------------
+
+WAIT_SOURCE = r"""
+#include "kv4_attention.cuh"
+
+// A warp waits for the first phase of an mbarrier, `limit` polls at most, and
+// each lane writes what it was told. `arrive`: the phase ends before the wait.
+__global__ void wait_kernel(unsigned limit, int arrive, int* told) {
+  __shared__ uint64_t bar;
+  const int lane = threadIdx.x;
+  if (lane == 0) {
+    lmcb::kv4::mbar_init(&bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (arrive) lmcb::kv4::mbar_arrive(&bar);
+  }
+  __syncwarp();
+  told[lane] = lmcb::kv4::warp_wait(&bar, 0, limit);
+}
+
+extern "C" int run_wait(unsigned limit, int arrive, int* told) {
+  wait_kernel<<<1, 32>>>(limit, arrive, told);
+  return cudaDeviceSynchronize();
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def wait_library(tmp_path_factory):
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    where = tmp_path_factory.mktemp("wait")
+    source, library = where / "wait.cu", where / "wait.so"
+    source.write_text(WAIT_SOURCE)
+    subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-shared",
+                    "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include"),
+                    "-I" + os.path.join(ROOT, "lmcache-ascend_b200", "csrc"), str(source), "-o",
+                    str(library)], check=True, timeout=300)
+    return ctypes.CDLL(str(library))
+
+
+@pytest.mark.parametrize("limit", [0, 1, 64])
+@pytest.mark.parametrize("arrive", [0, 1])
+def test_a_wait_tells_the_warp_one_thing(wait_library, arrive, limit):
+    """A wait that nobody answers gives up after its polls, for every lane, and
+    one whose phase has ended does not."""
+    told = torch.full((32,), -1, dtype=torch.int32, device=DEV)
+    assert wait_library.run_wait(limit, arrive, ctypes.c_void_p(told.data_ptr())) == 0
+    assert told.tolist() == [arrive if limit else 0] * 32
