@@ -535,10 +535,11 @@ __device__ __forceinline__ void qk_factors(const QkSource& src, const QkLane& ln
       w1 = j < E / 2 ? wa[2 * j] : wb[2 * j - E];
       w2 = j < E / 2 ? wa[2 * j + 1] : wb[2 * j - E + 1];
     }
+    const bool turn = kNeox || j < E / 2 ? ln.turn0 : ln.turn1;
     f.c1[j] = w1 * cs[j];
-    f.s1[j] = w1 * sn[j];
+    f.s1[j] = turn ? w1 * sn[j] : 0.0f;  // an infinite weight times 0 is NaN
     f.c2[j] = w2 * cs[j];
-    f.s2[j] = w2 * sn[j];
+    f.s2[j] = turn ? w2 * sn[j] : 0.0f;
   }
 }
 
@@ -560,10 +561,12 @@ __device__ __forceinline__ QkLane qk_lane(int l, int rot) {
 }
 
 // One head row, in a lane's two vectors: x becomes the result. All lanes of a
-// warp take part; `live` lanes hold something.
+// warp take part; `live` lanes hold something. Where nothing is rotated the partner
+// is left out, not multiplied by 0: it may be infinite. (A choice an element: two
+// paths, by lane or for rows with an infinity only, took 3 to 8% longer.)
 template <typename T, bool kNeox, int kLanes>
-__device__ __forceinline__ void qk_row(Vec16<T> (&x)[2], const QkFactors<T>& f, float mean,
-                                       float eps, bool live) {
+__device__ __forceinline__ void qk_row(Vec16<T> (&x)[2], const QkFactors<T>& f, const QkLane& ln,
+                                       float mean, float eps, bool live) {
   constexpr int E = 16 / sizeof(T);
   float x1[E], x2[E];  // the pairs
   float ss = 0.0f;
@@ -587,8 +590,10 @@ __device__ __forceinline__ void qk_row(Vec16<T> (&x)[2], const QkFactors<T>& f, 
   const float r = rsqrtf(fmaf(ss, mean, eps));
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const T y1 = from_f<T>(r * fmaf(x1[j], f.c1[j], -(x2[j] * f.s2[j])));
-    const T y2 = from_f<T>(r * fmaf(x2[j], f.c2[j], x1[j] * f.s1[j]));
+    const bool turn = kNeox || j < E / 2 ? ln.turn0 : ln.turn1;
+    const float from2 = turn ? x2[j] * f.s2[j] : 0.0f, from1 = turn ? x1[j] * f.s1[j] : 0.0f;
+    const T y1 = from_f<T>(r * fmaf(x1[j], f.c1[j], -from2));
+    const T y2 = from_f<T>(r * fmaf(x2[j], f.c2[j], from1));
     if constexpr (kNeox) {
       x[0].v[j] = y1;
       x[1].v[j] = y2;
@@ -698,7 +703,7 @@ qk_norm_rope_vec_kernel(const __grid_constant__ QkNormParams p, const uint32_t n
       asm volatile("cp.async.wait_group %0;" ::"n"(kQkAhead - 1) : "memory");
       V x[2] = {ring[slot][0][threadIdx.x], ring[slot][1][threadIdx.x]};
       if (++slot == kQkAhead) slot = 0;
-      qk_row<T, kNeox, kLanes>(x, f, mean, p.eps, live);
+      qk_row<T, kNeox, kLanes>(x, f, ln, mean, p.eps, live);
       if (live) {
         T* row = which ? static_cast<T*>(p.out[1]) + t * p.out_stride[1] +
                              static_cast<int64_t>(h - q_heads) * D

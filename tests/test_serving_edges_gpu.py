@@ -390,3 +390,50 @@ def test_a_wait_tells_the_warp_one_thing(wait_library, arrive, limit):
     told = torch.full((32,), -1, dtype=torch.int32, device=DEV)
     assert wait_library.run_wait(limit, arrive, ctypes.c_void_p(told.data_ptr())) == 0
     assert told.tolist() == [arrive if limit else 0] * 32
+
+
+# ---------------------------------------------------------------------------
+# qk_norm_rope: infinities and NaN
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("d,rot", [(128, 64), (128, 128), (64, 0), (256, 32), (80, 40), (72, 24)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_qk_not_finite(dtype, neox, d, rot, value):
+    """One element, or one weight, that is not finite, at every place: the
+    results are not finite exactly where the definition has it. Rows of
+    vectors and rows of elements (by the sizes) alike."""
+    cache = base.cos_sin(32, rot).to(DEV)
+    cache[:4] = base.cos_sin(36, rot)[32:].to(DEV)  # no angle 0: sin 0 times inf is no matter here
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(d, 1, d, generator=g).to(dtype)
+    pos = torch.randint(1, 32, (d,), generator=g).to(DEV)
+    q = x.clone()
+    q[torch.arange(d), 0, torch.arange(d)] = value  # row i: element i
+    q, k = q.to(DEV), x.to(DEV)
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    c_ops.qk_norm_rope(q, k, None, None, pos, cache, 1e-6, neox, qo, ko)
+    base.check_qk(ko, k, None, pos, cache, 1e-6, neox)
+
+    def same_kind(got, want):
+        got, want = got.cpu().double(), want.to(dtype).double()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.isinf(), want.isinf())
+        assert torch.equal(got[want.isinf()], want[want.isinf()])
+        return ~want.isnan() & ~want.isinf(), got, want
+
+    fine, got, want = same_kind(qo, ref.qk_norm_rope(q.cpu(), None, pos.cpu(), cache.cpu(), 1e-6,
+                                                     neox))
+    assert bool((got[fine] == 0).all()) and bool((want[fine] == 0).all())
+    for at in sorted({0, 1, rot // 2, max(rot - 1, 0), min(rot, d - 1), d - 2, d - 1}):
+        w = torch.ones(d)
+        w[at] = value
+        w = w.to(DEV)
+        c_ops.qk_norm_rope(k, k, w, None, pos, cache, 1e-6, neox, qo, ko)
+        want = ref.qk_norm_rope(k.cpu(), w.cpu(), pos.cpu(), cache.cpu(), 1e-6, neox)
+        fine, got, want = same_kind(qo, want)
+        rel = base.half_step(dtype) + (d / 2 + 16) * 2.0**-23
+        size = ref.qk_norm_rope(k.cpu(), None, pos.cpu(), cache.cpu(), 1e-6, neox).abs().amax(-1)
+        bound = rel * (want[fine].abs() + size.max()) + 2.0**-24
+        assert bool(((got[fine] - want[fine]).abs() <= bound).all())
