@@ -321,9 +321,15 @@ __device__ __forceinline__ void take_tile(const DecodeParams& p, const uint8_t* 
       vpar[u][i] = *reinterpret_cast<const uint32_t*>(vstage + tok * p.tok_stride + par_off);
       there[i] = true;
       if constexpr (!kAll) {
-        // what is not there may hold anything
+        // What is not there may hold anything. A V row whose parameters are no finite
+        // numbers (kv4_store writes none) gives NaN, by its K, to the queries that see
+        // it, and nothing to the others.
         there[i] = (valid[tok / 32] >> (tok % 32)) & 1;
         if (!there[i]) kpar[i] = vpar[u][i] = 0;
+        if ((vpar[u][i] & 0x7c00u) == 0x7c00u || (vpar[u][i] & 0x7c000000u) == 0x7c000000u) {
+          kpar[i] = 0x7e00u;
+          vpar[u][i] = 0;
+        }
       }
     }
 #pragma unroll

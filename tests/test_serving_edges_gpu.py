@@ -437,3 +437,29 @@ def test_qk_not_finite(dtype, neox, d, rot, value):
         size = ref.qk_norm_rope(k.cpu(), None, pos.cpu(), cache.cpu(), 1e-6, neox).abs().amax(-1)
         bound = rel * (want[fine].abs() + size.max()) + 2.0**-24
         assert bool(((got[fine] - want[fine]).abs() <= bound).all())
+
+
+# ---------------------------------------------------------------------------
+# Few query rows: value rows that are no numbers
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,group", [(64, 1), (64, 2), (128, 1), (256, 1)])
+def test_decode_not_finite_out_of_sight(dtype, d, group):
+    """Several queries in the decode kernel: a value row that is no number (a page
+    not made by kv4_store) spoils the queries that see it and no others."""
+    n, q = 40, 8
+    b = base.Batch([n], [q], 2, group, d, 16, dtype)
+    good = b.run()
+    for key in (33, 38):
+        slot = int(b.table[0, key // 16]) * 16 + key % 16
+        row = b.cache[1].view(-1, b.cache.shape[-1])[slot]
+        keep = row.clone()
+        for bad in (0x7E00, 0x7C00, 0x7E000000, 0x7C000000):  # s or z, NaN or infinite
+            row[2 * d // 8 : 2 * d // 8 + 2] = bad
+            out = b.run()
+            first = key - (n - q)  # the first query that sees it
+            assert bool((~out[first:].isfinite()).any(-1).all())
+            assert torch.equal(out[:first], good[:first])
+        row.copy_(keep)
+    assert torch.equal(b.run(), good)
