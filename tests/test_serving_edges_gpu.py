@@ -8,6 +8,7 @@ import shutil
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -463,3 +464,97 @@ def test_decode_not_finite_out_of_sight(dtype, d, group):
             assert torch.equal(out[:first], good[:first])
         row.copy_(keep)
     assert torch.equal(b.run(), good)
+
+
+# ---------------------------------------------------------------------------
+# Many query rows on streams and in graphs, and the ends of the shapes
+# ---------------------------------------------------------------------------
+
+def test_rows_on_streams_and_in_graphs():
+    """The kernel for many query rows with its cache split over CTAs: two graphs
+    replayed in turn, over new lengths too, and two streams at once."""
+    batches = [base.Batch([3000, 40], [30, 20], 1, 2, 128, 16, torch.bfloat16, seed=s)
+               for s in range(2)]
+    want = [b.run() for b in batches]
+    outs, graphs = [], []
+    for b in batches:
+        out, graph = torch.full_like(b.q, 3.0), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            b.run(out=out)
+        outs.append(out)
+        graphs.append(graph)
+    for _ in range(3):
+        for out, graph in zip(outs, graphs):
+            out.fill_(3.0)
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    b = batches[0]
+    b.lens_t.copy_(torch.tensor([1777, 25]))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    b.lens = [1777, 25]
+    b.codes = [[x[:n] for x in cs] for cs, n in zip(b.codes, b.lens)]
+    b.params = [[(s[:n], z[:n]) for s, z in ps] for ps, n in zip(b.params, b.lens)]
+    b.check(outs[0], rows=[0, 1, 15, 29])
+    b = base.Batch([3000, 40], [30, 20], 1, 2, 128, 16, torch.bfloat16, seed=0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for x, s in zip((b, batches[1]), streams):
+            with torch.cuda.stream(s):
+                got.append(x.run())
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert torch.equal(out, want[i % 2])
+    assert c_ops.device_status(0) == 0
+
+
+@pytest.mark.parametrize("qlen", [1, 17])
+def test_attention_most_requests(qlen):
+    """4096 requests, one of them long, most with one query, some without."""
+    rs = np.random.RandomState(qlen)
+    lens = rs.randint(1, 40, 4096)
+    lens[1234] = 900
+    qlens = np.minimum(rs.randint(0, qlen + 1, 4096), lens)
+    qlens[[0, 4095]] = 1
+    b = base.Batch([int(n) for n in lens], [int(n) for n in qlens], 1, 1, 64, 16, torch.float16,
+                   pad=2)
+    b.check(b.run(max_query=qlen), rows=[0, 5, -1])
+    assert c_ops.device_status(0) == 0
+
+
+@pytest.mark.parametrize("hkv,group,d", [(1, 4096, 64), (8, 512, 64), (128, 1, 64), (64, 1, 256),
+                                         (256, 16, 64)])
+def test_attention_most_heads(hkv, group, d):
+    """Up to 4096 query heads, over one KV head or many."""
+    b = base.Batch([70, 3], [1, 2], hkv, group, d, 16, torch.bfloat16)
+    out = b.run()
+    heads = sorted({0, 1, group - 1, group % (hkv * group), hkv * group // 2, hkv * group - 1})
+    at = 0
+    for r, n in enumerate(b.qlens):
+        for h in heads:
+            kv = h // group
+            pick = [[c[:, kv : kv + 1] for c in b.codes[r]],
+                    [(s[:, kv : kv + 1], z[:, kv : kv + 1]) for s, z in b.params[r]]]
+            pos = [b.lens[r] - n + i for i in range(n)]
+            want, slack = ref.kv4_attention(b.q[at : at + n, h : h + 1].cpu(), *pick, b.scale, pos,
+                                            0, 0, 1)
+            err = (out[at : at + n, h : h + 1].cpu().double() - want).abs()
+            assert bool((err <= 2.0**-8 * (want.abs() + slack) + slack).all())
+        at += n
+    assert c_ops.device_status(0) == 0
+
+
+@pytest.mark.parametrize("qlens,max_query", [([1, 1, 1], 40), ([2, 0, 3], 64), ([1, 1, 1], 3)])
+def test_attention_longer_promises(qlens, max_query):
+    """A promised length that no request reaches, pages of 1024 tokens, a block
+    table that is part of a wider one, and rows behind the last request."""
+    b = base.Batch([700, 5, 1030], qlens, 2, 4, 128, 1024, torch.bfloat16, pad=5)
+    wide = torch.full((3, b.table.shape[1] + 7), -5, dtype=torch.int32, device=DEV)
+    wide[:, 3 : 3 + b.table.shape[1]] = b.table
+    b.table = wide[:, 3 : 3 + b.table.shape[1]]
+    out = b.run(max_query=max_query, starts=b.starts, max_len=5000)
+    b.check(out)
+    assert c_ops.device_status(0) == 0
