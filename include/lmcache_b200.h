@@ -386,7 +386,9 @@ LMCB_API int lmcb_rotary_embedding_k_fused(const void* oldPositions, const void*
  *   slotMapping, positions  [numTokens] of slotType, out. Token i of request b
  *                  is entry queryStart[b] + i: its position is contextLens[b] +
  *                  i, its slot page * blockSize + position % blockSize, or -1
- *                  (which the transfers skip) where it has no page. Entries
+ *                  (which the transfers skip) where it has no page or (with
+ *                  LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE) the slot does not fit
+ *                  slotType. Entries
  *                  behind the last request: slot -1, position 0.
  *   queryStart     [numRequests + 1] int32, out: first entry of each request
  *   seqLens        [numRequests] int32, out: contextLens + queryLens
@@ -467,7 +469,8 @@ LMCB_API int lmcb_kv4_load(const int32_t* kvCache, int64_t numBlocks, int64_t bl
  *   queryStart     [batch + 1] int32: request b's queries are rows
  *                  queryStart[b] ... queryStart[b + 1], the last of them at
  *                  position seqLens[b] - 1. NULL: row b is request b's one query.
- *   maxQueryLen    no request has more queries (a larger one is left out and flagged)
+ *   maxQueryLen    no request has more queries (a larger one is left out and
+ *                  flagged; 0: no request has any, and nothing is launched)
  *   maxSeqLen      how long requests are expected to be: sizes the launch only
  *   scale          factor of q . k before the softmax
  *   window, sinks  window > 0: a query sees the last `window` keys up to its own
@@ -479,7 +482,16 @@ LMCB_API int lmcb_kv4_load(const int32_t* kvCache, int64_t numBlocks, int64_t bl
  * they were. Keys on pages outside the cache are not seen and set
  * LMCB_DEVICE_FLAG_SLOT_OUT_OF_RANGE; lengths outside [0, tableCols * blockSize]
  * count as 0, and a queryStart that leaves [0, numQueryRows] or descends gives
- * its request no queries; both set LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE. */
+ * its request no queries; both set LMCB_DEVICE_FLAG_LENGTH_OUT_OF_RANGE.
+ * Precision: logits are fp32 sums of exact products; sums and the softmax are
+ * fp32, with the GPU's approximate exponential and reciprocal. Rounded to fp16 are,
+ * up to 16 query rows a KV head (8 with heads of 256), each p s of a weight and a V
+ * scale; beyond, each weight p and each value z + s c, where values in the same 16
+ * tokens as one 2^21 times larger have fewer bits (fp16 results take p as two fp16
+ * numbers). Logits of 2^24 and more, which fp32 does not tell apart, may give NaN;
+ * rows of the cache whose scale or zero is no finite number give NaN or infinities
+ * to the queries that see them, and to no others. Calls of the same sizes and
+ * inputs give the same bits. */
 LMCB_API int lmcb_kv4_attention(const void* query, int type, int64_t queryTokenStride,
                                 int64_t numQueryRows, const int32_t* kvCache, int64_t numBlocks,
                                 int64_t blockSize, const int32_t* blockTable, int64_t tableStride,

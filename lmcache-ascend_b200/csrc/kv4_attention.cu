@@ -40,7 +40,7 @@
 // leave no CTA idle; a second kernel joins requests that were cut.
 //
 // Measured: 96 requests of up to 16384 tokens, 8 KV heads of 128, 4 query heads
-// each, bf16: 201 us, 4.1 TB/s of cache rows (0.63 of a plain copy). Issue slots
+// each, bf16: 204 us, 4.0 TB/s of cache rows (0.63 of a plain copy). Issue slots
 // bound it (60% used, with two CTAs an SM that is what their dependences leave):
 // 313 instructions a warp for 16 tokens of a head, a third of them masks and
 // shifts of codes. A warp that only brings tiles cost 222 us, loads straight from

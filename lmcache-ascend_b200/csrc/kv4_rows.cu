@@ -23,9 +23,9 @@
 // down to 2^-21 of 2^7 are normal; V is normal down to 2^-28 of the largest of
 // its 16 tokens. Further apart, values in the 16 of a larger one lose bits (2^24
 // apart, those that bf16 does not have). Exact codes as V, with s in P and z in a
-// sum of its own, would not: they took 1370 to 1450 us where this takes 1140, for
-// what every pair of tokens then has to load. So would more head for P cost time:
-// 2^9 instead of 2^7, with more tiles taken again, 1194 us.
+// sum of its own, would not: they took 1280 us where this takes 1100, for what
+// every pair of tokens then has to load and add. More head for P costs time too:
+// with 2^9 instead of 2^7 more tiles are taken again, 5% of the time.
 //
 // A CTA has two such units (one for D = 256), 256 query rows, which share the
 // tiles. Per tile the tensor core needs 1024 cycles for them, the exponentials
@@ -43,15 +43,19 @@
 // its m then leaves room for 2^8 more.
 //
 // Measured: 4 suffixes of up to 1024 tokens behind prefixes of up to 16384, 64
-// query heads over 8 of 128, bf16: 1150 us, 700 TFLOP/s (0.42 of a plain bf16
-// product). By its counters no one unit bounds it: 54% of the issue slots, 32% of
-// the tensor pipe. It waits in the chain from S through softmax to P V, of which
-// a CTA has two units' worth under way. Q K^T with 64 columns takes 46
-// cycles of the tensor core where 32 would do (128 columns: 64.5), but two units'
-// S of 128 and O do not fit its memory. On the way: one unit a CTA 1856 us, two
-// 1513, eight softmax warps a unit instead of four 1455, one elected lane in the
-// issuing warp instead of a branch by lane 1191, pairs of fp32 1150; eight warps
-// that bring instead of four 1380 (fewer registers for softmax).
+// query heads over 8 of 128, bf16: 1091 us, 736 TFLOP/s (0.44 of a plain bf16
+// product). By its counters no one unit bounds it: 58% of the issue slots, 37% of
+// the tensor pipe. Nor does one of its parts: with K and V not written at all it
+// takes 970 us, without the exponentials 1092, without both 905. What is left is
+// the chain of waits from S through softmax to P V, of which a CTA has two units'
+// worth under way. Q K^T with 64 columns takes 46 cycles of the tensor core where
+// 32 would do (128 columns: 64.5); two S of 128 columns a unit do not fit beside its
+// O, one would, without Q K^T running ahead in its unit. On the way: one unit a CTA
+// 1856 us, two 1513, eight softmax warps a unit instead of four 1455, one elected
+// lane that issues products instead of a branch by lane 1191, pairs of fp32 1150, one
+// thread for the whole loop of products and a reference a row 1091; eight warps that
+// bring instead of four 1380 (fewer registers for softmax). The compiler's schedule
+// of softmax alone moved it by 8% both ways between forms with the same instructions.
 #include <climits>
 #include <type_traits>
 

@@ -612,7 +612,7 @@ __device__ __forceinline__ void qk_row(Vec16<T> (&x)[2], const QkFactors<T>& f, 
 // So a lane brings its vectors of the next kQkAhead steps, of the next items
 // too, by asynchronous copies into places of its own in shared memory, which
 // nobody else reads: there is nothing to wait for but its own copies.
-// Measured for 16384 tokens of 64 + 8 heads of 128 (bf16, 604 MB): 104 us, 0.89
+// Measured for 16384 tokens of 64 + 8 heads of 128 (bf16, 604 MB): 107 us, 0.88
 // of the copy bandwidth; with two steps ahead in registers, or a ring of whole
 // tokens by bulk copies, 147 us. Bound by memory.
 constexpr int kQkAhead = 6;
