@@ -452,8 +452,10 @@ LMCB_API int lmcb_kv4_store(const void* key, const void* value, int type, int64_
                             int64_t blockSize, const void* slotMapping, int slotType,
                             int64_t numTokens, int64_t numHeads, int64_t headSize, void* stream);
 
-/* The values of the rows of slotMapping, in fp32, bf16 or fp16. Rows of
- * skipped slots (as in lmcb_kv4_store) are left as they were. */
+/* The values of the rows of slotMapping, in fp32, bf16 or fp16, rounded once (in
+ * fp16 a value beyond 65504 is infinite: z + 15 s of a row that spans the whole
+ * range may be). Rows of skipped slots (as in lmcb_kv4_store) are left as they
+ * were. */
 LMCB_API int lmcb_kv4_load(const int32_t* kvCache, int64_t numBlocks, int64_t blockSize,
                            const void* slotMapping, int slotType, void* key, void* value,
                            int type, int64_t keyTokenStride, int64_t valueTokenStride,

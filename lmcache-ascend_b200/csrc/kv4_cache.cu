@@ -3,9 +3,11 @@
 //
 // A head row x of D values keeps z = fp16(min x), s = fp16((max x - min x) / 15)
 // and the codes clamp(rne((x - z) / s), 0, 15); it reads back as z + s c.
-// Difference and quotient are fp32, each rounded once; s and z are fp16 because an attention kernel multiplies by them in fp32
-// anyway and a row's 4 bytes are then 1/17 of its 68 (D = 128). NaN counts as 0 and values
-// beyond the fp16 range as its ends, so that every row is finite.
+// Difference and quotient are fp32, each rounded once; s and z are fp16 because an
+// attention kernel multiplies by them in fp32 anyway and a row's 4 bytes are then
+// 1/17 of its 68 (D = 128). NaN counts as 0 and values beyond the fp16 range as its
+// ends, so that s and z are finite, and with them every value in fp32 and bf16 (in
+// fp16 z + 15 s of a row that spans the whole range may round to infinity).
 //
 // The code is the exact one, see word_of: it depends on no rounding of a
 // reciprocal and equals that of any exact computation.
@@ -15,8 +17,8 @@
 // 16-byte access of a 16-bit type), and a lane has up to kMost rows in flight.
 //
 // Measured, 40001 tokens of 8 heads of 128 in bf16 (208 MB each way): load 37 us,
-// 5.6 TB/s, bound by memory; store 72 us, 2.9 TB/s, bound by issue slots (75%
-// of them used: 174 instructions a warp for two head rows, of which half find the
+// 5.6 TB/s, bound by memory; store 73 us, 2.8 TB/s, bound by issue slots (76%
+// of them used: 176 instructions a warp for two head rows, of which half find the
 // codes and the sixth part the row's minimum and maximum). With a division per
 // element instead of the corrected product it took 215 us.
 #include <cuda_bf16.h>
