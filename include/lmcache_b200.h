@@ -434,9 +434,9 @@ LMCB_API int lmcb_qk_norm_rope(const void* query, const void* key, int type,
  * (word h * D / 8 + w: values 8 w ... 8 w + 7 of head h, value 8 w + j in bits
  * 4 j ... 4 j + 3), then one word a head: fp16 scale s in the low half, fp16
  * zero z in the high half. A code c stands for z + s c, with z = fp16(min),
- * s = fp16((max - min) / 15) of the head's values (difference and quotient fp32,
- * rounded once each) and the nearest code, ties to even; NaN is kept as 0, values
- * beyond the fp16 range as its ends. W is that length rounded up to four words, so a
+ * s = fp16((max - min) * r), r the fp32 number nearest to 1 / 15, of the head's
+ * values and the nearest code, ties to even; NaN is kept as 0, values beyond
+ * the fp16 range as its ends. W is that length rounded up to four words, so a
  * 4-bit cache moves through the transfers above as rows of W int32 (type
  * LMCB_DTYPE_INT32, hiddenDims W). */
 

@@ -1,13 +1,15 @@
 // kv4_cache.cu -- rows into and out of the paged KV cache held in 4 bits
 // (kv4_store, kv4_load; layout in kv4.cuh).
 //
-// A head row x of D values keeps z = fp16(min x), s = fp16((max x - min x) / 15)
-// and the codes clamp(rne((x - z) / s), 0, 15); it reads back as z + s c.
-// Difference and quotient are fp32, each rounded once; s and z are fp16 because an
-// attention kernel multiplies by them in fp32 anyway and a row's 4 bytes are then
-// 1/17 of its 68 (D = 128). NaN counts as 0 and values beyond the fp16 range as its
-// ends, so that s and z are finite, and with them every value in fp32 and bf16 (in
-// fp16 z + 15 s of a row that spans the whole range may round to infinity).
+// A head row x of D values keeps z = fp16(min x), s = fp16((max x - min x) r), r the
+// fp32 number nearest to 1 / 15, and the codes clamp(rne((x - z) / s), 0, 15); it
+// reads back as z + s c. Difference and product are fp32, each rounded once (a
+// quotient by 15 gives another fp16 number for one fp32 row in 8,700); s and z are
+// fp16 because an attention kernel multiplies by them in fp32 anyway and a row's 4
+// bytes are then 1/17 of its 68 (D = 128). NaN counts as 0 and values beyond the
+// fp16 range as its ends, so that s and z are finite, and with them every value in
+// fp32 and bf16 (in fp16 z + 15 s of a row that spans the whole range may round to
+// infinity).
 //
 // The code is the exact one, see word_of: it depends on no rounding of a
 // reciprocal and equals that of any exact computation.
@@ -213,22 +215,9 @@ __device__ __forceinline__ uint32_t word_of(const float (&v)[8], const Coder& c,
   return word - kBias;
 }
 
-// The fp32 quotient x / 15, rounded once, as a product with 1 / 15 in two parts:
-// x h + (x l), h = fp32(1 / 15), l = fp32(1 / 15 - h) (Brisebarre, Muller and Raina,
-// "Accelerating correctly rounded floating-point division when the divisor is known
-// in advance", IEEE Transactions on Computers 53(8), 2004). Their conditions leave a
-// few mantissas to try for a divisor; all 2^23 were, and agree. A plain
-// product with h is off by a step for two quotients of three.
-__device__ __forceinline__ float fifteenth(float x) {
-  constexpr double kExact = 1.0 / 15.0;
-  constexpr float kHigh = static_cast<float>(kExact);
-  constexpr float kLow = static_cast<float>(kExact - static_cast<double>(kHigh));
-  return __fmaf_rn(x, kHigh, __fmul_rn(x, kLow));
-}
-
 // z and s of a head row whose values are in [lo, hi].
 __device__ __forceinline__ void row_params(float lo, float hi, float& z, float& s) {
-  s = __half2float(__float2half_rn(fifteenth(hi - lo)));
+  s = __half2float(__float2half_rn(__fmul_rn(hi - lo, 1.0f / 15.0f)));
   // + 0: a zero of either sign is kept as +0, so equal rows have equal words
   z = __half2float(__float2half_rn(lo)) + 0.0f;
 }

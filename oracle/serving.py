@@ -63,8 +63,9 @@ def kv4_quantise(x):
     x = x.double()
     x = torch.where(x.isnan(), torch.zeros_like(x), x).clamp(-HALF_MAX, HALF_MAX)
     lo, hi = x.min(-1).values, x.max(-1).values
-    span = (hi - lo).float()                       # fp32 difference and quotient,
-    scale = (span.double() / 15.0).float().half().double()        # each rounded once
+    span = (hi - lo).float()                       # fp32 difference and product,
+    fifteenth = torch.tensor(1.0 / 15.0, dtype=torch.float32).double()
+    scale = (span.double() * fifteenth).float().half().double()   # each rounded once
     zero = lo.float().half().double() + 0.0        # never -0
     q = (x - zero[..., None]) / torch.where(scale > 0, scale, torch.ones_like(scale))[..., None]
     codes = torch.where(scale[..., None] > 0, q.round().clamp(0, 15), torch.zeros_like(q))
